@@ -623,6 +623,53 @@ void q4_cuda_mmq_q8_compat(int on);
 bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const int8_t **q, const float **d,
                              const int32_t **sums);
 
+/* ---------------- 4-bit floating point: MXFP4 and NVFP4 ----------------
+ * The formats that the B200's tensor cores multiply as they are (no reference counterpart: the engine's formats are integer
+ * ones; these are the counterparts of q4_mmq_quantize, q4_cuda_mmq_swiglu_quantize, q4_mmvq_n and q4_mmq_mul_id for them).
+ * A value is a sign and a magnitude out of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (E2M1) times its block's scale:
+ *   Q4_T_MXFP4  32 values share 2^(byte - 127); byte 255 = NaN
+ *   Q4_T_NVFP4  16 values share an e4m3 number; byte 0x7f = NaN.  A factor for a whole matrix, where there is one, is
+ *               the caller's and goes into the products' scale
+ * Quantising v = x * mul (rounded to fp32): MXFP4 takes the power of two floor(log2 max|v|) - 2 (-127 at least), NVFP4 the
+ * e4m3 number nearest to max|v| / 6 (448 at most; a block that this rounds to 0 is zeros); codes are the nearest, ties to even, 6
+ * for all beyond it.  A block with an infinity or a NaN becomes NaN.
+ * cols: a multiple of 32, at most 65536; any number of rows below 2^31.  A quantised matrix is an opaque
+ * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned, in one of two forms:
+ *   Q4_FP4_ROWS     activations: what the products take as d_xq
+ *   Q4_FP4_WEIGHTS  weights: what they take as d_w; the matrices of several experts stand a stride apart
+ *   put              n_mat matrices of a checkpoint -> weights at d_w + i * stride.  d_codes [n_mat][rows][cols / 2], value 2 i
+ *                    in the low half of byte i; d_scales [n_mat][rows][cols / 32 or 16].  d_scales == NULL (MXFP4): d_codes
+ *                    holds ggml blocks of 17 bytes, the scale first, values j and j + 16 in the halves of byte j
+ *   quantize         fp32 rows, ld_x floats apart, -> either form
+ *   swiglu_quantize  silu(gu[r][k]) * gu[r][n_ff + k] * mul -> rows form.  The codes are those of the exact values (one
+ *                    that fp32 leaves next to a border is computed again in 64 bits)
+ *   values           either form -> the fp32 values that it stands for
+ *   mul              d_y[t][r] = scale * W[r] . x[t], ld_y floats apart; rows is the one that d_xq was made with
+ *   mul_id           row p of d_dst, for expert e's p in [bounds[e], bounds[e + 1]) (device int32, n_expert + 1 entries, ascending;
+ *                    only p below total_rows), = scale * d_expert_scale[e] * W_e . x[d_rows[p]]; d_expert_scale NULL = 1, d_rows NULL
+ *                    = p itself, an entry of d_rows outside [0, xq_rows) counts as a row of zeros.  Rows of d_dst that no
+ *                    expert has are left alone.  n_expert <= 1024
+ * Sums are fp32; products of codes are exact.  Outputs may not overlap inputs. */
+#define Q4_T_MXFP4 39u
+#define Q4_T_NVFP4 40u
+#define Q4_FP4_ROWS 0u
+#define Q4_FP4_WEIGHTS 1u
+uint64_t q4_cuda_fp4_bytes(uint32_t type, uint32_t form, uint64_t rows, uint64_t cols);
+bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uint8_t *d_scales, uint64_t rows, uint64_t cols,
+                     uint64_t n_mat, void *d_w, uint64_t stride);
+bool q4_cuda_fp4_quantize(uint32_t type, uint32_t form, const float *d_x, uint64_t ld_x, float mul, uint64_t rows,
+                          uint64_t cols, void *d_q);
+bool q4_cuda_fp4_swiglu_quantize(uint32_t type, const float *d_gu, uint64_t ld_gu, float mul, uint64_t rows,
+                                 uint64_t n_ff, void *d_hq);
+bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q, uint64_t rows, uint64_t cols, float *d_out,
+                        uint64_t ld_out);
+bool q4_cuda_fp4_mul(uint32_t type, const void *d_w, uint64_t w_rows, uint64_t w_cols, const void *d_xq, uint64_t rows,
+                     float scale, float *d_y, uint64_t ld_y);
+bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_rows, uint64_t w_cols, uint64_t expert_stride_bytes,
+                        uint32_t n_expert, const void *d_xq, uint64_t xq_rows, const int32_t *d_rows,
+                        const int32_t *d_bounds, uint64_t total_rows, float scale, const float *d_expert_scale,
+                        float *d_dst, uint64_t ld_dst);
+
 /* Seeded synthetic tensors generated on the device (benchmark and smoke
  * support, no reference counterpart): n_blocks IQ3_S super-blocks with
  * fp16 d = |N(0,1)| * 2^-6 and uniform random payload bytes; n fp32 values

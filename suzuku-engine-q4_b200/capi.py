@@ -211,6 +211,13 @@ SIGNATURES = {
     "q4_cuda_mmq_tc_mode": (b, [C.c_int]),
     "q4_cuda_mmq_q8_compat": (None, [C.c_int]),
     "q4_cuda_mmq_q8_sections": (b, [vp, u64, u64, vp, vp, vp]),
+    "q4_cuda_fp4_bytes": (u64, [u32, u32, u64, u64]),
+    "q4_cuda_fp4_put": (b, [u32, vp, vp, u64, u64, u64, vp, u64]),
+    "q4_cuda_fp4_quantize": (b, [u32, u32, vp, u64, f32, u64, u64, vp]),
+    "q4_cuda_fp4_swiglu_quantize": (b, [u32, vp, u64, f32, u64, u64, vp]),
+    "q4_cuda_fp4_values": (b, [u32, u32, vp, u64, u64, vp, u64]),
+    "q4_cuda_fp4_mul": (b, [u32, vp, u64, u64, vp, u64, f32, vp, u64]),
+    "q4_cuda_fp4_mul_id": (b, [u32, vp, u64, u64, u64, u32, vp, u64, vp, vp, u64, f32, vp, vp, u64]),
     "q4_cuda_synth_iq3s": (b, [vp, u64, u64]),
     "q4_cuda_synth_iq3s_at": (b, [vp, u64, u64, u64]),
     "q4_cuda_synth_normal": (b, [vp, u64, u64, f32, f32]),
