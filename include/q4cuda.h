@@ -670,6 +670,19 @@ bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_rows, uint64_
                         const int32_t *d_bounds, uint64_t total_rows, float scale, const float *d_expert_scale,
                         float *d_dst, uint64_t ld_dst);
 
+/* How evenly a router spreads its tokens (no reference counterpart).  d_logits [n_tok][n_exp] are the router's, d_ids
+ * [n_tok][topk] the picks of q4_hip_route_pf (an id outside [0, n_exp) is no pick); d_valid [n_tok] (bytes; NULL = all)
+ * is 0 for padding, which counts for nothing.  With n tokens that count, f_e = counts_e / (n topk), p_t = softmax(logits_t) and
+ * P_e = (1 / n) sum_t p_te:
+ *   d_counts [n_exp] picks of each expert;  d_prob [n_exp] = P;  d_loss [1] = coef * n_exp * sum_e f_e P_e
+ *   d_dlogits [n_tok][n_exp] = g * d loss / d logits = g coef n_exp / n * p_tj (f_j - sum_e f_e p_te), zeros for padding;
+ *   g = *d_gout (NULL: 1); d_dlogits may be d_logits
+ * Any of the four may be NULL.  n_exp <= 1024, topk <= 64, n_tok < 2^23.  A row whose logits are all -inf has no
+ * probabilities and no gradient; without any token that counts all results are zeros.  The same inputs give the same bits. */
+bool q4_cuda_route_balance(const float *d_logits, const int32_t *d_ids, const uint8_t *d_valid, uint32_t n_tok,
+                           uint32_t n_exp, uint32_t topk, float coef, const float *d_gout, int32_t *d_counts,
+                           float *d_prob, float *d_loss, float *d_dlogits);
+
 /* Seeded synthetic tensors generated on the device (benchmark and smoke
  * support, no reference counterpart): n_blocks IQ3_S super-blocks with
  * fp16 d = |N(0,1)| * 2^-6 and uniform random payload bytes; n fp32 values

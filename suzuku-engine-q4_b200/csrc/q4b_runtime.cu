@@ -24,6 +24,8 @@ void q4b_elem_shutdown();
 bool q4b_mmvq_warm();    // q4b_mmvq.cu: quantised rows of the dense 8-bit product
 bool q4b_route_small_warm();   // q4b_decode.cu: counters of the one-launch routing
 void q4b_route_small_shutdown();
+bool q4b_balance_warm();       // q4b_balance.cu: sums of the balance loss
+void q4b_balance_shutdown();
 void q4b_mmvq_shutdown();
 bool q4b_wbuf_tiled(const void *p);
 bool q4b_router_tc_warm();   // q4b_router.cu: shared-memory limit of the batch router product
@@ -245,7 +247,8 @@ bool alloc_scratch() {
     Q4B_CHECK(cudaMalloc(&s.hbuf, nq * sizeof(float)));
     q4b_router_tc_warm();
     q4b_mmq_tc_warm();  // without it the grouped product stays on the CUDA cores
-    return q4b_fused_warm() && q4b_window_warm() && q4b_elem_warm() && q4b_mmvq_warm() && q4b_route_small_warm();
+    return q4b_fused_warm() && q4b_window_warm() && q4b_elem_warm() && q4b_mmvq_warm() && q4b_route_small_warm() &&
+           q4b_balance_warm();
 }
 
 }  // namespace
@@ -349,6 +352,7 @@ extern "C" void q4_hip_shutdown(void) {
     q4b_elem_shutdown();
     q4b_mmvq_shutdown();
     q4b_route_small_shutdown();
+    q4b_balance_shutdown();
     q4b_fused_shutdown();
     q4b_stack_forget_host(nullptr);
     cudaFree(s.xq);
