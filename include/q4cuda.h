@@ -647,7 +647,7 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  *   mul              d_y[t][r] = scale * W[r] . x[t], ld_y floats apart; rows is the one that d_xq was made with
  *   mul_id           row p of d_dst, for expert e's p in [bounds[e], bounds[e + 1]) (device int32, n_expert + 1 entries, ascending;
  *                    only p below total_rows), = scale * d_expert_scale[e] * W_e . x[d_rows[p]]; d_expert_scale NULL = 1, d_rows NULL
- *                    = p itself, an entry of d_rows outside [0, xq_rows) counts as a row of zeros.  Rows of d_dst that no
+ *                    = p itself, an entry of d_rows outside [0, xq_rows) gives a row of zeros.  Rows of d_dst that no
  *                    expert has are left alone.  n_expert <= 1024
  * Sums are fp32; products of codes are exact.  Outputs may not overlap inputs. */
 #define Q4_T_MXFP4 39u

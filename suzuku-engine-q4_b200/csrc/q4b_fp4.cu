@@ -344,7 +344,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) few_k(const MArgs a) 
             e = lo;
         }
         const uint64_t xr = a.rows ? (uint64_t)(uint32_t)a.rows[p] : p;
-        const bool there = xr < a.x_rows;       // a row that is not there counts as zeros
+        const bool there = xr < a.x_rows;       // a row that is not there gives zeros
         const uint8_t *w = a.w + e * a.stride;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t c = lane * 32u; c < a.cols; c += 1024u) {
@@ -384,7 +384,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) few_k(const MArgs a) 
         for (int j = 0; j < 4; j++) {
             const float y = q4b_warp_sum(acc[j]);
             const uint32_t r = r0 + 32u * j;
-            if (lane == 0 && r < a.w_rows) a.dst[p * a.ld + r] = y * f;
+            if (lane == 0 && r < a.w_rows) a.dst[p * a.ld + r] = there ? y * f : 0.f;
         }
     }
 }
@@ -432,8 +432,11 @@ bool quantize(uint32_t type, uint32_t form, const float *x, uint64_t ld, float m
     return q4b_launch_ok("fp4 quantize");
 }
 
+bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
+
 bool product(uint32_t type, MArgs &a) {
     OnDevice dev;
+    if (a.total > 4u) return tc_product(type == NV, a);
     const dim3 grid((a.w_rows + 127u) / 128u * 4u, (unsigned)(a.total < 65535u ? a.total : 65535u));
     if (type == NV) q4b_launch(few_k<true>, grid, dim3(256), 0, g_q4b.stream, a);
     else q4b_launch(few_k<false>, grid, dim3(256), 0, g_q4b.stream, a);
