@@ -9,6 +9,8 @@
 // follow one another (128 values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there):
 //   rows     [word][row]: a product's activation tiles begin at any row, or gather their rows
 //   weights  [row / 128][word][row % 32][row / 32 % 4]: 512 bytes that go to tensor memory as they are
+#include <type_traits>
+
 namespace fp4 {
 
 constexpr uint32_t MX = 39u, NV = 40u;      // ggml type ids
@@ -75,35 +77,48 @@ template <bool NVF> __device__ __forceinline__ uint32_t scale_byte(float a) {
     const int e = (int)(__float_as_uint(a) >> 23) - 2;      // 127 + floor(log2 a) - 2 for a normal a, at most 252
     return (uint32_t)max(e, 0);
 }
-// Eight values of a block with that scale to codes.  MXFP4: the product with the inverse power of two is exact.  NVFP4: a quotient
-// by the scale, rounded, falls on a border between two codes only where the exact one does (as above: the scale
-// has four bits, a border three).
+// What a block's values are multiplied with to become units of its scale: exact in MXFP4 (a power of two), rounded in NVFP4; 0 where
+// the scale is 0 or NaN, whose codes are 0.
+template <bool NVF> __device__ __forceinline__ float inverse(uint32_t sb) {
+    if (NVF) return sb == 0u || sb == 0x7fu ? 0.f : __frcp_rn(e4m3_value(sb));
+    return sb == 255u ? 0.f : __uint_as_float((254u - sb) << 23);
+}
+// Eight values of a block with that scale to codes.  MXFP4: the product with the inverse power of two is exact.  NVFP4: the quotient
+// by the scale is rounded correctly (Markstein 1990: a product with the rounded inverse, corrected once by its exact remainder), and then
+// falls on a border between two codes only where the exact one does (as above: the scale has four bits, a border three).
 template <bool NVF> __device__ __forceinline__ uint32_t codes8(const float *v, uint32_t sb) {
+    const float inv = inverse<NVF>(sb);
     float t[8];
     if (NVF) {
-        if (sb == 0u || sb == 0x7fu) return 0u;
+        if (inv == 0.f) return 0u;
         const float s = e4m3_value(sb);
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = __fdiv_rn(v[i], s);
+        for (int i = 0; i < 8; i++) {
+            const float q = v[i] * inv;
+            t[i] = fmaf(fmaf(-q, s, v[i]), inv, q);
+        }
     } else {
-        if (sb == 255u) return 0u;
-        const float inv = __uint_as_float((254u - sb) << 23);
+        if (inv == 0.f) return 0u;
 #pragma unroll
         for (int i = 0; i < 8; i++) t[i] = v[i] * inv;
     }
     return encode8(t);
 }
-__device__ __forceinline__ float max8(const float *v) {   // NaN where one of them is none
-    float a = 0.f;
-    bool bad = false;
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN where one of them is none
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max8(const float *v) {
+    float a = fabsf(v[0]);
 #pragma unroll
-    for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(v[i])), bad |= v[i] != v[i];
-    return bad ? __uint_as_float(0x7fc00000u) : a;
+    for (int i = 1; i < 8; i++) a = max_nan(a, fabsf(v[i]));
+    return a;
 }
 // Largest of the lanes that hold a block (two with 16 values, four with 32), NaN if one is: as the bits of magnitudes,
 // whose order is the numbers' and in which NaN is largest.
 template <bool NVF> __device__ __forceinline__ float block_max(float a) {
-    uint32_t u = __float_as_uint(a);
+    uint32_t u = __float_as_uint(a) & 0x7fffffffu;
     u = max(u, __shfl_xor_sync(0xffffffffu, u, 1));
     if (!NVF) u = max(u, __shfl_xor_sync(0xffffffffu, u, 2));
     return __uint_as_float(u);
@@ -119,8 +134,8 @@ struct QArgs {
     uint8_t *codes, *scales;
 };
 
-__device__ __forceinline__ void load8(const float *p, bool vec, float *v) {
-    if (vec) {
+template <bool VEC> __device__ __forceinline__ void load8(const float *p, float *v) {
+    if (VEC) {
         const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
@@ -129,11 +144,9 @@ __device__ __forceinline__ void load8(const float *p, bool vec, float *v) {
     }
 }
 
-// silu(g) u mul, and whether its fp32 value is too close to something to decide by: borders are looked for later,
-// here only what fp32 cannot hold.
 __device__ __forceinline__ double swiglu64(double g, double u, double mul) { return g / (1.0 + exp(-g)) * u * mul; }
 
-// The same steps as above in 64 bits, for a block in which fp32 leaves a doubt.
+// The scale and the codes of a block in 64 bits.
 template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uint32_t &sb) {
     double a = 0.0;
     bool bad = false;
@@ -170,121 +183,149 @@ template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uin
     return c;
 }
 
-// A warp takes 256 values of a row, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same columns
-// of eight rows that follow one another, whose scale words lie side by side in the rows order.
-template <bool NVF, bool WF, bool SWIGLU> __global__ void __launch_bounds__(256) quantize_k(const QArgs a, bool vec) {
+// A warp takes 256 values of a row at a time, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same
+// columns of eight rows that follow one another, whose scale words lie side by side in the rows order; U such pieces of a row are
+// loaded before the first is quantised.
+template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
+    constexpr int U = SWIGLU ? 1 : 2;
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint64_t row = (uint64_t)blockIdx.x * 8u + warp;
     if (row >= a.rows) return;
-    for (uint32_t c0 = blockIdx.y * 256u; c0 < a.cols; c0 += gridDim.y * 256u) {
+    const float *const src = a.x + row * a.ld;
+    uint8_t *const codes = a.codes + row * (a.cols >> 1);
+    auto store = [&](uint32_t c0, uint32_t q, uint32_t sb) {
         const uint32_t c = c0 + lane * 8u;
         const bool live = c < a.cols;       // cols is a multiple of 32: a block is whole or not there
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const float *p = a.x + row * a.ld + c;
-        uint32_t sb, q;
-        if (!SWIGLU) {
-            if (live) load8(p, vec, v);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] *= a.mul;
-            sb = scale_byte<NVF>(block_max<NVF>(max8(v)));
-            q = codes8<NVF>(v, sb);
-        } else {
-            float g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (live) load8(p, vec, g), load8(p + a.cols, vec, u);
-            // fp32 is off by at most 2 steps for the exponential, half a step each for the sum, the quotient and the two
-            // products, and as much again where a half step counts double: 2^-21 is more than that.
-            constexpr float D = 4.76837158203125e-7f;
-            float lo[8], hi[8];
-            bool doubt = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = __fdiv_rn(g[i], 1.f + expf(-g[i])) * u[i] * a.mul;
-                lo[i] = fmaf(v[i], -D, v[i]), hi[i] = fmaf(v[i], D, v[i]);
-                doubt |= g[i] < -80.f || fabsf(v[i]) > 1e38f;       // the exponential, or the product, leaves fp32's range
-            }
-            const float top = max8(v);
-            sb = scale_byte<NVF>(block_max<NVF>(top));
-            q = codes8<NVF>(v, sb);
-            const float lo_top = block_max<NVF>(max8(lo)), hi_top = block_max<NVF>(max8(hi));
-            doubt |= scale_byte<NVF>(lo_top) != sb || scale_byte<NVF>(hi_top) != sb || codes8<NVF>(lo, sb) != q ||
-                     codes8<NVF>(hi, sb) != q || (hi_top > 0.f && hi_top < 1e-30f);
-            if (__any_sync(0xffffffffu, doubt)) {
-                double w[8];
-                for (int i = 0; i < 8; i++) w[i] = swiglu64(g[i], u[i], a.mul);
-                q = exact8<NVF>(w, sb);
-            }
-        }
-        if (live) *reinterpret_cast<uint32_t *>(a.codes + row * (a.cols >> 1) + (c >> 1)) = q;
+        if (live) *reinterpret_cast<uint32_t *>(codes + (c >> 1)) = q;
         // four blocks' bytes to a word: 8 lanes (NVFP4) or 16
         uint32_t w = live ? sb << (8u * (NVF ? (lane >> 1) & 3u : (lane >> 2) & 3u)) : 0u;
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 2 : 4);
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 4 : 8);
         if ((lane & (NVF ? 7u : 15u)) == 0u)
             *reinterpret_cast<uint32_t *>(a.scales + word_at<WF>(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words, a.pitch)) = w;
-    }
-}
-
-// A quantised matrix as the values that it stands for: eight a thread.
-template <bool NVF, bool WF> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t pitch,
-                                                                            uint32_t cols, uint32_t words, float *out, uint64_t ld, bool vec) {
-    q4b_pdl_wait();
-    const uint32_t per = cols >> 3;
-    const uint64_t n = rows * per, step = (uint64_t)gridDim.x * blockDim.x;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const uint64_t row = i / per;
-        const uint32_t c = (uint32_t)(i - row * per) * 8u, b = c >> (NVF ? 4 : 5);
-        const float s = scale_value<NVF>(scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)]) * 0.5f;
-        const uint32_t q = *reinterpret_cast<const uint32_t *>(codes + row * (cols >> 1) + (c >> 1));
-        const uint32_t m[2] = {prmt(MAG_LO, MAG_HI, q & 0x7777u), prmt(MAG_LO, MAG_HI, (q >> 16) & 0x7777u)};
-        float v[8];
+    };
+    const uint32_t step = gridDim.y * 256u;
+    for (uint32_t c0 = blockIdx.y * 256u; c0 < a.cols; c0 += U * step) {
+        float v[U][8], u[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float f = (float)((m[k >> 2] >> (8 * (k & 3))) & 0xffu) * s;
-            v[k] = (q >> (4 * k)) & 8u ? -f : f;
+        for (int k = 0; k < U; k++) {
+            const uint32_t c = c0 + k * step + lane * 8u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[k][i] = 0.f, u[i] = 0.f;
+            if (c < a.cols) load8<VEC>(src + c, v[k]);
+            if (SWIGLU && c < a.cols) load8<VEC>(src + a.cols + c, u);
         }
-        float *o = out + row * ld + c;
-        if (vec) {
-            reinterpret_cast<float4 *>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        if (!SWIGLU) {
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                if (k && c0 + k * step >= a.cols) break;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[k][i] *= a.mul;
+                const uint32_t sb = scale_byte<NVF>(block_max<NVF>(max8(v[k])));
+                store(c0 + k * step, codes8<NVF>(v[k], sb), sb);
+            }
         } else {
+            // fp32 is off by at most 2 steps of 2^-23 for the exponential, half a one for the sum, 2 for the quotient (its divisor is
+            // below 2^126), half a one each for two products and for the unit's, 1 for its inverse: below 2^-20.  Where that leaves
+            // the scale or a code in doubt, or fp32's range is left, the warp computes in 64 bits.
+            constexpr float LO = 1.f - 0x1p-20f, HI = 1.f + 0x1p-20f;
+            float t[8];
+            bool doubt = false;
 #pragma unroll
-            for (int k = 0; k < 8; k++) o[k] = v[k];
+            for (int i = 0; i < 8; i++) {
+                const float g = v[0][i];
+                t[i] = __fdividef(g, 1.f + expf(-g)) * u[i] * a.mul;
+                doubt |= g < -80.f;
+            }
+            const float top = block_max<NVF>(max8(t));
+            uint32_t sb = scale_byte<NVF>(top * LO);
+            doubt |= scale_byte<NVF>(top * HI) != sb || top > 1e38f || (top > 0.f && top < 1e-30f);
+            const float inv = inverse<NVF>(sb);
+            float lo[8], hi[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) lo[i] = t[i] * (inv * LO), hi[i] = t[i] * (inv * HI);
+            uint32_t q = encode8(lo);
+            doubt |= q != encode8(hi) && inv != 0.f;
+            if (inv == 0.f) q = 0u;
+            if (__any_sync(0xffffffffu, doubt)) {
+                double w[8];
+                for (int i = 0; i < 8; i++) w[i] = swiglu64(v[0][i], u[i], a.mul);
+                q = exact8<NVF>(w, sb);
+            }
+            store(c0, q, sb);
         }
     }
 }
 
-// Matrices in the form of a checkpoint to the weights order: a thread takes a row's word of scales and its codes.  scales == NULL:
-// ggml blocks of 17 bytes, the scale and then codes j (low half) and j + 16 (high half) in byte j.
-template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint32_t cols, uint32_t words,
-                                                                 uint64_t n_mat, uint8_t *w, uint64_t stride, uint64_t scale_off) {
+// A quantised matrix as the values that it stands for: a warp 256 values of a row at a time.
+template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows,
+                                                                                      uint64_t pitch, uint32_t cols, uint32_t words, float *out, uint64_t ld) {
     q4b_pdl_wait();
-    constexpr uint32_t B = NVF ? 16u : 32u;
-    const uint32_t nb = cols / B;
-    const uint64_t n = n_mat * rows * words, step = (uint64_t)gridDim.x * blockDim.x;
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t row = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
+    if (row >= rows) return;
+#pragma unroll 2
+    for (uint32_t c0 = blockIdx.y * 256u; c0 < cols; c0 += gridDim.y * 256u) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++) {          // four values a lane, so that a store is whole lines
+            const uint32_t c = c0 + h * 128u + lane * 4u;
+            if (c >= cols) continue;
+            const uint32_t b = c >> (NVF ? 4 : 5);
+            const float s = scale_value<NVF>(scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)]) * 0.5f;
+            const uint32_t q = *reinterpret_cast<const uint16_t *>(codes + row * (cols >> 1) + (c >> 1));
+            const uint32_t m = prmt(MAG_LO, MAG_HI, q & 0x7777u);
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = (float)((m >> (8 * k)) & 0xffu) * s;
+                v[k] = (q >> (4 * k)) & 8u ? -f : f;
+            }
+            float *o = out + row * ld + c;
+            if (VEC) *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            else o[0] = v[0], o[1] = v[1], o[2] = v[2], o[3] = v[3];
+        }
+    }
+}
+
+// Matrices in the form of a checkpoint to the weights order: a thread takes 16 bytes of codes (32 values), and the one that has a
+// word's first block its scales.  scales == NULL: ggml blocks of 17 bytes, the scale and then codes j (low half) and j + 16 (high half)
+// in byte j.
+template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *codes, const uint8_t *scales, uint32_t rows, uint32_t cols, uint32_t words,
+                                                                 uint8_t *w, uint64_t stride, uint64_t scale_off, bool vec) {
+    q4b_pdl_wait();
+    constexpr uint32_t PER = NVF ? 2u : 4u;          // pieces of 32 values to a word of scales
+    const uint32_t pieces = words * PER, nb = cols / (NVF ? 16u : 32u);
+    const uint64_t n = (uint64_t)rows * pieces, step = (uint64_t)gridDim.x * blockDim.x;
+    const uint64_t r0 = (uint64_t)blockIdx.y * rows;
+    uint8_t *const to = w + blockIdx.y * stride;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const uint32_t wd = (uint32_t)(i % words);
-        const uint64_t r = i / words, mat = r / rows, row = r - mat * rows;
-        uint32_t sw = 0;
-        uint8_t *to = w + mat * stride + row * (cols >> 1);
-        for (uint32_t j = 0; j < 4u; j++) {
-            const uint32_t b = wd * 4u + j;
-            if (b >= nb) break;
-            if (scales) {
-                sw |= (uint32_t)scales[r * nb + b] << (8u * j);
-                const uint8_t *s = codes + r * (cols >> 1) + b * (B / 2u);
-                for (uint32_t k = 0; k < B / 2u; k++) to[b * (B / 2u) + k] = s[k];
-            } else {
-                const uint8_t *s = codes + (r * nb + b) * 17u;
-                sw |= (uint32_t)s[0] << (8u * j);
-                for (uint32_t k = 0; k < 8u; k++) {       // values 2 k, 2 k + 1 and 16 further
-                    const uint32_t p = s[1u + 2u * k], q = s[2u + 2u * k];
-                    to[b * 16u + k] = (uint8_t)((p & 15u) | (q << 4));
-                    to[b * 16u + 8u + k] = (uint8_t)((p >> 4) | (q & 0xf0u));
-                }
+        const uint32_t row = (uint32_t)(i / pieces), p = (uint32_t)(i - (uint64_t)row * pieces);
+        const uint64_t r = r0 + row;
+        if (p % PER == 0u) {
+            uint32_t sw = 0;
+            for (uint32_t j = 0; j < 4u; j++) {
+                const uint32_t b = p / PER * 4u + j;
+                if (b < nb) sw |= (uint32_t)(scales ? scales[r * nb + b] : codes[(r * nb + b) * 17u]) << (8u * j);
+            }
+            *reinterpret_cast<uint32_t *>(to + scale_off + word_at<true>(row, p / PER, words, 0)) = sw;
+        }
+        if (p * 32u >= cols) continue;
+        uint32_t q[4] = {0, 0, 0, 0};
+        if (scales && vec) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(codes + r * (cols >> 1) + p * 16u);
+            q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w;
+        } else if (scales) {
+            for (uint32_t k = 0; k < 16u; k++) q[k >> 2] |= (uint32_t)codes[r * (cols >> 1) + p * 16u + k] << (8u * (k & 3u));
+        } else {
+            const uint8_t *s = codes + (r * nb + p) * 17u + 1u;
+            for (uint32_t k = 0; k < 8u; k++) {       // values 2 k, 2 k + 1 and 16 further
+                const uint32_t a = s[2u * k], b = s[2u * k + 1u];
+                q[k >> 2] |= ((a & 15u) | ((b & 15u) << 4)) << (8u * (k & 3u));
+                q[2u + (k >> 2)] |= ((a >> 4) | (b & 0xf0u)) << (8u * (k & 3u));
             }
         }
-        *reinterpret_cast<uint32_t *>(w + mat * stride + scale_off + word_at<true>(row, wd, words, 0)) = sw;
+        *reinterpret_cast<uint4 *>(to + (uint64_t)row * (cols >> 1) + p * 16u) = make_uint4(q[0], q[1], q[2], q[3]);
     }
 }
 
@@ -420,14 +461,17 @@ bool quantize(uint32_t type, uint32_t form, const float *x, uint64_t ld, float m
     a.scales = a.codes + code_bytes(rows, a.cols);
     const bool vec = aligned(x, 16) && ld % 4u == 0;
     OnDevice dev;
-    const dim3 grid((unsigned)((rows + 7u) / 8u), (a.cols + 255u) / 256u);
-    if (type == NV) {
-        if (form == WEIGHTS) q4b_launch(quantize_k<true, true, SWIGLU>, grid, dim3(256), 0, g_q4b.stream, a, vec);
-        else q4b_launch(quantize_k<true, false, SWIGLU>, grid, dim3(256), 0, g_q4b.stream, a, vec);
-    } else {
-        if (form == WEIGHTS) q4b_launch(quantize_k<false, true, SWIGLU>, grid, dim3(256), 0, g_q4b.stream, a, vec);
-        else q4b_launch(quantize_k<false, false, SWIGLU>, grid, dim3(256), 0, g_q4b.stream, a, vec);
-    }
+    // a row's pieces of 256 values to one warp while there are rows enough for all SMs
+    const uint32_t groups = (uint32_t)((rows + 7u) / 8u), pieces = (a.cols + 255u) / 256u;
+    const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
+    const dim3 grid(groups, pieces < want ? pieces : want);
+    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, a); };
+    auto pick = [&](auto nv, auto wf) {
+        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
+        vec ? go(quantize_k<N, W, SWIGLU, true>) : go(quantize_k<N, W, SWIGLU, false>);
+    };
+    if (SWIGLU || form == ROWS) type == NV ? pick(std::true_type(), std::false_type()) : pick(std::false_type(), std::false_type());
+    else type == NV ? pick(std::true_type(), std::bool_constant<!SWIGLU>()) : pick(std::false_type(), std::bool_constant<!SWIGLU>());
     g_q4b_launches++;
     return q4b_launch_ok("fp4 quantize");
 }
@@ -458,13 +502,14 @@ extern "C" bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uin
         return false;
     OnDevice dev;
     const uint32_t words = n_words(type == NV, (uint32_t)cols);
-    const uint64_t n = n_mat * rows * words, want = (n + 255u) / 256u, most = (uint64_t)g_q4b.n_sm * 16u;
-    const dim3 grid((unsigned)(want < most ? want : most));
+    const uint64_t n = rows * words * (type == NV ? 2u : 4u), want = (n + 255u) / 256u, most = ((uint64_t)g_q4b.n_sm * 16u + n_mat - 1u) / n_mat;
+    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)n_mat);
     const uint64_t off = code_bytes(rows, (uint32_t)cols);
-    if (type == NV)
-        q4b_launch(put_k<true>, grid, dim3(256), 0, g_q4b.stream, d_codes, d_scales, rows, (uint32_t)cols, words, n_mat, (uint8_t *)d_w, stride, off);
-    else
-        q4b_launch(put_k<false>, grid, dim3(256), 0, g_q4b.stream, d_codes, d_scales, rows, (uint32_t)cols, words, n_mat, (uint8_t *)d_w, stride, off);
+    const bool vec = aligned(d_codes, 16);
+    auto go = [&](auto k) {
+        q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, d_codes, d_scales, (uint32_t)rows, (uint32_t)cols, words, (uint8_t *)d_w, stride, off, vec);
+    };
+    type == NV ? go(put_k<true>) : go(put_k<false>);
     g_q4b_launches++;
     return q4b_launch_ok("fp4 put");
 }
@@ -486,18 +531,17 @@ extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q
     if (!g_q4b.ok || !shape(type, rows, cols) || form > WEIGHTS || !d_q || !d_out || ld_out < cols || !aligned(d_q, 16) || !aligned(d_out, 4)) return false;
     OnDevice dev;
     const uint8_t *codes = (const uint8_t *)d_q, *scales = codes + code_bytes(rows, (uint32_t)cols);
-    const uint64_t n = rows * (cols / 8u), want = (n + 255u) / 256u, most = (uint64_t)g_q4b.n_sm * 16u, pitch = row_pitch(rows);
-    const dim3 grid((unsigned)(want < most ? want : most));
-    const bool vec = aligned(d_out, 16) && ld_out % 4u == 0;
-    const uint32_t c = (uint32_t)cols, words = n_words(type == NV, c);
-    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, pitch, c, words, d_out, ld_out, vec); };
-    if (type == NV) {
-        if (form == WEIGHTS) go(values_k<true, true>);
-        else go(values_k<true, false>);
-    } else {
-        if (form == WEIGHTS) go(values_k<false, true>);
-        else go(values_k<false, false>);
-    }
+    const uint64_t pitch = row_pitch(rows);
+    const uint32_t c = (uint32_t)cols, words = n_words(type == NV, c), groups = (uint32_t)((rows + 7u) / 8u), pieces = (c + 255u) / 256u;
+    const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
+    const dim3 grid(groups, pieces < want ? pieces : want);
+    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, pitch, c, words, d_out, ld_out); };
+    auto pick = [&](auto nv, auto wf) {
+        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
+        aligned(d_out, 16) && ld_out % 4u == 0 ? go(values_k<N, W, true>) : go(values_k<N, W, false>);
+    };
+    if (form == WEIGHTS) type == NV ? pick(std::true_type(), std::true_type()) : pick(std::false_type(), std::true_type());
+    else type == NV ? pick(std::true_type(), std::false_type()) : pick(std::false_type(), std::false_type());
     g_q4b_launches++;
     return q4b_launch_ok("fp4 values");
 }
