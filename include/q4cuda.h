@@ -634,9 +634,10 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  * e4m3 number nearest to max|v| / 6 (448 at most; a block that this rounds to 0 is zeros); codes are the nearest, ties to even, 6
  * for all beyond it.  A block with an infinity or a NaN becomes NaN.
  * cols: a multiple of 32, at most 65536; any number of rows below 2^31.  A quantised matrix is an opaque
- * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned, in one of two forms:
+ * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned.  form says what it is for:
  *   Q4_FP4_ROWS     activations: what the products take as d_xq
  *   Q4_FP4_WEIGHTS  weights: what they take as d_w; the matrices of several experts stand a stride apart
+ * (the bytes of both are in the same order, so that a product of two activations is one call, too)
  *   put              n_mat matrices of a checkpoint -> weights at d_w + i * stride.  d_codes [n_mat][rows][cols / 2], value 2 i
  *                    in the low half of byte i; d_scales [n_mat][rows][cols / 32 or 16].  d_scales == NULL (MXFP4): d_codes
  *                    holds ggml blocks of 17 bytes, the scale first, values j and j + 16 in the halves of byte j

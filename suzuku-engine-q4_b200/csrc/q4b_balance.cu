@@ -7,7 +7,7 @@
 // f is known before the logits are looked at, so that loss and gradient are one pass over them.
 namespace balance {
 
-constexpr uint32_t MAX_E = 1024u;
+constexpr uint32_t MAX_E = 1024u, CL = 8u;      // experts; CTAs of a cluster
 struct Args {
     const float *logits;
     const int32_t *ids;
@@ -17,10 +17,8 @@ struct Args {
     const float *gout;
     int32_t *counts;
     float *prob, *loss, *dlogits;
-    int32_t *hist;        // [count CTA][1 + n_exp]: tokens that count, picks of every expert
-    uint32_t n_hist;      // 0: the one CTA of rows_k counts by itself
-    float *part;          // [CTA][n_exp] sums of probabilities
-    uint32_t *done;       // CTAs of rows_k that are through
+    float *part;          // [cluster][n_exp] sums of probabilities
+    uint32_t *done;       // CTAs that are through
 };
 
 // Picks of a slice of the tokens, with shared-memory counters; returns after a barrier.
@@ -28,97 +26,128 @@ __device__ __forceinline__ void count(const Args &a, uint32_t cta, uint32_t ctas
     for (uint32_t i = threadIdx.x; i < a.n_exp; i += blockDim.x) hist[i] = 0;
     if (threadIdx.x == 0) *n_live = 0;
     __syncthreads();
-    const uint32_t n = a.n_tok * a.topk, step = ctas * blockDim.x, at = cta * blockDim.x + threadIdx.x;       // below 2^29
-    for (uint32_t i = at; i < n; i += step) {
-        const int32_t e = a.ids[i];
-        if ((uint32_t)e < a.n_exp && (!a.valid || a.valid[i / a.topk])) atomicAdd(&hist[e], 1);
-    }
     int32_t live = 0;
-    for (uint32_t t = at; t < a.n_tok; t += step) live += !a.valid || a.valid[t];
+    for (uint32_t t = cta * blockDim.x + threadIdx.x; t < a.n_tok; t += ctas * blockDim.x) {
+        const bool ok = !a.valid || a.valid[t];
+        live += ok;
+        const int32_t *ids = a.ids + (uint64_t)t * a.topk;
+        for (uint32_t k0 = 0; k0 < a.topk; k0 += 16u) {
+            int32_t e[16];
+#pragma unroll
+            for (uint32_t k = 0; k < 16u; k++) e[k] = k0 + k < a.topk ? ids[k0 + k] : -1;
+#pragma unroll
+            for (uint32_t k = 0; k < 16u; k++)
+                if (ok && (uint32_t)e[k] < a.n_exp) atomicAdd(&hist[e[k]], 1);
+        }
+    }
     live = __reduce_add_sync(0xffffffffu, live);
     if ((threadIdx.x & 31u) == 0 && live) atomicAdd(n_live, live);
     __syncthreads();
 }
-__global__ void __launch_bounds__(1024) count_k(const Args a) {
-    __shared__ int32_t hist[MAX_E], n_live;
-    q4b_pdl_wait();
-    count(a, blockIdx.x, gridDim.x, hist, &n_live);
-    int32_t *o = a.hist + (uint64_t)blockIdx.x * (1u + a.n_exp);
-    if (threadIdx.x == 0) o[0] = n_live;
-    for (uint32_t i = threadIdx.x; i < a.n_exp; i += blockDim.x) o[1u + i] = hist[i];
+// A value of another CTA's shared memory, by this CTA's address of it.
+__device__ __forceinline__ uint32_t peer_word(const void *p, uint32_t cta) {
+    uint32_t a, v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A warp takes a token's row at a time, 32 NV experts in registers (VEC: four neighbours a lane and load); its sums of
-// probabilities stay there too.  They are added up in a fixed order: over the warps of a CTA in shared memory, over the CTAs by
-// the last one to come to its end.  Bound by the reads of the logits and the writes of the gradient: 32 warps an SM have
-// a row each in flight.
-template <int NV, bool VEC> __global__ void __launch_bounds__(NV > 16 ? 512 : 1024) rows_k(const Args a) {
-    constexpr uint32_t W = NV > 16 ? 16u : 32u, N = NV * 32u;
+// 2^x to 2 steps of 2^-23; x is a rounded multiple of log2(e), off by |x| 2^-24: a probability that matters has a small one.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// One launch.  Every cluster of eight CTAs counts all picks, an eighth a CTA, and adds the eighths up through distributed shared
+// memory.  Then a warp takes a token's row at a time, 32 NV experts in registers (VEC: four neighbours a lane and load); its sums
+// of probabilities stay there too.  They are added up in a fixed order: over the warps of a CTA in shared memory, over the
+// CTAs of a cluster (each takes an eighth of the experts), over the clusters by the last CTA to come to its end.
+// Warps of a CTA: as many as have registers for a row and its sums.
+__host__ __device__ constexpr uint32_t warps(int nv) { return nv > 16 ? 16u : nv > 4 ? 24u : 32u; }
+template <int NV, bool VEC> __global__ void __launch_bounds__(32u * warps(NV)) rows_k(const Args a) {
+    constexpr uint32_t W = warps(NV), N = NV * 32u;
     __shared__ __align__(16) float f[N];
     __shared__ __align__(16) float sum[W / 2u][N];
-    __shared__ int32_t hist[N], n_live;
+    __shared__ int32_t hist[N], total[N], n_here;
     __shared__ float red[W];
     __shared__ bool last;
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     auto at = [&](int i) { return VEC ? (uint32_t)(i >> 2) * 128u + lane * 4u + (i & 3u) : (uint32_t)i * 32u + lane; };   // expert of register i
-    if (a.n_hist) {
-        for (uint32_t e = threadIdx.x; e <= a.n_exp; e += blockDim.x) {
-            int32_t s = 0;
-#pragma unroll 8
-            for (uint32_t c = 0; c < a.n_hist; c++) s += a.hist[(uint64_t)c * (1u + a.n_exp) + e];
-            if (e == 0) n_live = s;
-            else hist[e - 1u] = s;
+    float p[NV];
+    auto load = [&](uint32_t t) {             // (padding is read, too: nobody waits for its mark)
+        if (t >= a.n_tok) return;
+        const float *row = a.logits + (uint64_t)t * a.n_exp;
+        if (VEC) {
+#pragma unroll
+            for (int i = 0; i < NV; i += 4) {
+                float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (at(i) < a.n_exp) v = *reinterpret_cast<const float4 *>(row + at(i));
+                p[i] = v.x, p[i + 1] = v.y, p[i + 2] = v.z, p[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; i++) p[i] = at(i) < a.n_exp ? row[at(i)] : -INFINITY;
         }
-        __syncthreads();
-    } else {
-        count(a, 0, 1, hist, &n_live);
-    }
+    };
+    const uint32_t rank = blockIdx.x % CL, clusters = gridDim.x / CL, step = gridDim.x * W;
+    uint32_t t = blockIdx.x * W + warp;
+    load(t);                                  // the first row comes while the picks are counted
+    count(a, rank, CL, hist, &n_here);
+    cluster_sync();
+    int32_t n_live = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < CL; c++) n_live += (int32_t)peer_word(&n_here, c);
     const float inv_n = n_live ? 1.f / (float)n_live : 0.f, share = n_live ? 1.f / ((float)n_live * (float)a.topk) : 0.f;
-    for (uint32_t i = threadIdx.x; i < N; i += blockDim.x) f[i] = i < a.n_exp ? (float)hist[i] * share : 0.f;
+    for (uint32_t i = threadIdx.x; i < N; i += blockDim.x) {
+        int32_t n = 0;
+        if (i < a.n_exp)
+#pragma unroll
+            for (uint32_t c = 0; c < CL; c++) n += (int32_t)peer_word(&hist[i], c);
+        total[i] = n;
+        f[i] = (float)n * share;
+    }
     __syncthreads();
     const float g = (a.gout ? *a.gout : 1.f) * a.coef * (float)a.n_exp * inv_n;
     float acc[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) acc[i] = 0.f;
-    for (uint32_t t = blockIdx.x * W + warp; t < a.n_tok; t += gridDim.x * W) {
-        const float *row = a.logits + (uint64_t)t * a.n_exp;
+    for (; t < a.n_tok; t += step, load(t)) {
         const bool live = !a.valid || a.valid[t];
-        float p[NV], m = -INFINITY;
-        if (VEC) {
-#pragma unroll
-            for (int i = 0; i < NV; i += 4) {
-                float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (live && at(i) < a.n_exp) v = *reinterpret_cast<const float4 *>(row + at(i));
-                p[i] = v.x, p[i + 1] = v.y, p[i + 2] = v.z, p[i + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NV; i++) p[i] = live && at(i) < a.n_exp ? row[at(i)] : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; i++) m = fmaxf(m, p[i]);
-        m = q4b_warp_max(m);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            p[i] = m == -INFINITY && p[i] == p[i] ? 0.f : expf(p[i] - m);      // a row without any expert has no probabilities
-            s += p[i];
-        }
-        s = q4b_warp_sum(s);
-        const float inv = s == 0.f ? 0.f : 1.f / s;
-        float inner = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            p[i] *= inv;
-            acc[i] += p[i];
-            inner = fmaf(p[i], f[at(i)], inner);
-        }
-        if (!a.dlogits) continue;
-        inner = q4b_warp_sum(inner);
         float *d = a.dlogits + (uint64_t)t * a.n_exp;
+        if (live) {
+            float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; i++) p[i] = live ? g * p[i] * (f[at(i)] - inner) : 0.f;
+            for (int i = 0; i < NV; i++) m = fmaxf(m, p[i]);
+            m = q4b_warp_max(m);
+            if (m == -INFINITY) m = 0.f;              // a row without any expert: all exponentials are 0
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                p[i] = exp2_approx((p[i] - m) * 1.4426950408889634f);
+                s += p[i];
+            }
+            s = q4b_warp_sum(s);
+            const float inv = s == 0.f ? 0.f : __fdiv_rn(1.f, s);
+            float inner = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                p[i] *= inv;
+                acc[i] += p[i];
+                inner = fmaf(p[i], f[at(i)], inner);
+            }
+            if (!a.dlogits) continue;
+            inner = q4b_warp_sum(inner);
+#pragma unroll
+            for (int i = 0; i < NV; i++) p[i] = g * p[i] * (f[at(i)] - inner);
+        } else {
+            if (!a.dlogits) continue;
+#pragma unroll
+            for (int i = 0; i < NV; i++) p[i] = 0.f;
+        }
         if (VEC) {
 #pragma unroll
             for (int i = 0; i < NV; i += 4)
@@ -139,39 +168,38 @@ template <int NV, bool VEC> __global__ void __launch_bounds__(NV > 16 ? 512 : 10
         for (int i = 0; i < NV; i++) sum[warp][at(i)] += acc[i];
     }
     __syncthreads();
-    const bool alone = gridDim.x == 1u;
     for (uint32_t e = threadIdx.x; e < a.n_exp; e += blockDim.x) {
         float s = 0.f;
 #pragma unroll
         for (uint32_t w = 0; w < W / 2u; w++) s += sum[w][e];
-        if (alone) sum[0][e] = s;           // (a column is one thread's)
-        else a.part[(uint64_t)blockIdx.x * a.n_exp + e] = s;
+        sum[0][e] = s;           // (a column is one thread's)
+    }
+    cluster_sync();
+    const bool alone = clusters == 1u;
+    const uint32_t slice = (a.n_exp + CL - 1u) / CL, e0 = alone ? 0u : rank * slice, e1 = alone ? (rank ? 0u : a.n_exp) : min(e0 + slice, a.n_exp);
+    for (uint32_t e = e0 + threadIdx.x; e < e1; e += blockDim.x) {
+        float s = 0.f;
+#pragma unroll
+        for (uint32_t c = 0; c < CL; c++) s += __uint_as_float(peer_word(&sum[0][e], c));
+        if (alone) sum[1][e] = s;
+        else a.part[(uint64_t)(blockIdx.x / CL) * a.n_exp + e] = s;
     }
     if (!alone) {
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) last = atomicInc(a.done, gridDim.x - 1u) == gridDim.x - 1u;     // back at 0 behind the last one
-        __syncthreads();
-        if (!last) return;
-        __threadfence();
-        // W / 2 groups of threads add up a run of the CTAs' sums each, then the groups' are added
-        const uint32_t grp = warp >> 1, run = (gridDim.x + W / 2u - 1u) / (W / 2u), c0 = grp * run, c1 = min(c0 + run, gridDim.x);
-        for (uint32_t e = (warp & 1u) * 32u + lane; e < a.n_exp; e += 64u) {
-            float s = 0.f;
-#pragma unroll 10
-            for (uint32_t c = c0; c < c1; c++) s += __ldcg(a.part + (uint64_t)c * a.n_exp + e);
-            sum[grp][e] = s;
-        }
     }
-    __syncthreads();
+    cluster_sync();              // nobody reads a CTA that has gone
+    if (alone ? rank != 0u : !last) return;
+    __threadfence();
     float l = 0.f;
     for (uint32_t e = threadIdx.x; e < a.n_exp; e += blockDim.x) {
-        float s = sum[0][e];
+        float s = alone ? sum[1][e] : 0.f;
         if (!alone)
-#pragma unroll
-            for (uint32_t w = 1; w < W / 2u; w++) s += sum[w][e];
+#pragma unroll 8
+            for (uint32_t c = 0; c < clusters; c++) s += __ldcg(a.part + (uint64_t)c * a.n_exp + e);
         const float p = s * inv_n;
-        if (a.counts) a.counts[e] = hist[e];
+        if (a.counts) a.counts[e] = total[e];
         if (a.prob) a.prob[e] = p;
         l = fmaf(f[e], p, l);
     }
@@ -184,28 +212,51 @@ template <int NV, bool VEC> __global__ void __launch_bounds__(NV > 16 ? 512 : 10
     }
 }
 
-constexpr uint32_t MAX_HIST = 32u;
-static int32_t *g_hist = nullptr;
 static uint32_t *g_done = nullptr;
 static float *g_part = nullptr;
+static uint32_t g_clusters = 0;       // that run at a time
+
+template <int NV, bool VEC> bool launch(const Args &a, uint32_t clusters, uint32_t *most) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CL * clusters);
+    cfg.blockDim = dim3(32u * warps(NV));
+    cfg.stream = g_q4b.stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CL, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    if (most) {
+        int n = 0;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, rows_k<NV, VEC>, &cfg) != cudaSuccess || n < 1) return false;
+        *most = (uint32_t)n;
+        return true;
+    }
+    (void)cudaLaunchKernelEx(&cfg, rows_k<NV, VEC>, a);
+    g_q4b_launches++;
+    return q4b_launch_ok("route balance");
+}
 }  // namespace balance
 
 // The sums' scratch, once: calls come one after another on the library's stream.
 bool q4b_balance_warm() {
     using namespace balance;
-    if (g_hist) return true;
+    if (g_done) return true;
+    uint32_t n = 0;
+    if (!launch<16, true>(Args{}, 1u, &n)) return false;
+    Q4B_CHECK(cudaMalloc(&g_part, (size_t)n * MAX_E * sizeof(float)));
     Q4B_CHECK(cudaMalloc(&g_done, 256));
     Q4B_CHECK(cudaMemset(g_done, 0, 256));
-    Q4B_CHECK(cudaMalloc(&g_part, (size_t)g_q4b.n_sm * MAX_E * sizeof(float)));
-    Q4B_CHECK(cudaMalloc(&g_hist, (size_t)MAX_HIST * (1u + MAX_E) * sizeof(int32_t)));
+    g_clusters = n;
     return true;
 }
 void q4b_balance_shutdown() {
     using namespace balance;
-    cudaFree(g_hist);
     cudaFree(g_done);
     cudaFree(g_part);
-    g_hist = nullptr;
     g_done = nullptr;
     g_part = nullptr;
 }
@@ -213,26 +264,14 @@ void q4b_balance_shutdown() {
 extern "C" bool q4_cuda_route_balance(const float *d_logits, const int32_t *d_ids, const uint8_t *d_valid, uint32_t n_tok, uint32_t n_exp, uint32_t topk,
                                       float coef, const float *d_gout, int32_t *d_counts, float *d_prob, float *d_loss, float *d_dlogits) {
     using namespace balance;
-    if (!g_q4b.ok || !g_hist || !d_logits || !d_ids || !n_tok || n_tok > 0x7fffffu || !n_exp || n_exp > MAX_E || !topk || topk > 64u ||
+    if (!g_q4b.ok || !g_done || !d_logits || !d_ids || !n_tok || n_tok > 0x7fffffu || !n_exp || n_exp > MAX_E || !topk || topk > 64u ||
         (((uintptr_t)d_logits | (uintptr_t)d_ids | (uintptr_t)d_gout | (uintptr_t)d_counts | (uintptr_t)d_prob | (uintptr_t)d_loss | (uintptr_t)d_dlogits) & 3u))
         return false;
     fp4::OnDevice dev;
-    Args a = {d_logits, d_ids, d_valid, n_tok, n_exp, topk, coef, d_gout, d_counts, d_prob, d_loss, d_dlogits, g_hist, 0u, g_part, g_done};
-    const uint32_t sm = (uint32_t)g_q4b.n_sm, warps = n_exp > 512u ? 16u : 32u;
-    uint32_t ctas = (n_tok + warps - 1u) / warps;
-    if (ctas > sm) ctas = sm;
-    if (n_tok <= 4u * warps) ctas = 1;       // up to four rows a warp: one CTA, one launch
-    if (ctas > 1u) {
-        a.n_hist = (n_tok * topk + 2047u) / 2048u;
-        if (a.n_hist > MAX_HIST) a.n_hist = MAX_HIST;
-        q4b_launch(count_k, dim3(a.n_hist), dim3(1024), 0, g_q4b.stream, a);
-        g_q4b_launches++;
-    }
+    const Args a = {d_logits, d_ids, d_valid, n_tok, n_exp, topk, coef, d_gout, d_counts, d_prob, d_loss, d_dlogits, g_part, g_done};
+    const uint32_t rows = CL * (n_exp > 512u ? warps(32) : n_exp > 128u ? warps(16) : warps(4)), want = (n_tok + rows - 1u) / rows, n = want < g_clusters ? want : g_clusters;
     const bool vec = n_exp % 4u == 0 && (((uintptr_t)d_logits | (uintptr_t)d_dlogits) & 15u) == 0;
-    auto go = [&](auto k) { q4b_launch(k, dim3(ctas), dim3(32u * warps), 0, g_q4b.stream, a); };
-    if (n_exp <= 128u) vec ? go(rows_k<4, true>) : go(rows_k<4, false>);
-    else if (n_exp <= 512u) vec ? go(rows_k<16, true>) : go(rows_k<16, false>);
-    else vec ? go(rows_k<32, true>) : go(rows_k<32, false>);
-    g_q4b_launches++;
-    return q4b_launch_ok("route balance");
+    if (n_exp <= 128u) return vec ? launch<4, true>(a, n, nullptr) : launch<4, false>(a, n, nullptr);
+    if (n_exp <= 512u) return vec ? launch<16, true>(a, n, nullptr) : launch<16, false>(a, n, nullptr);
+    return vec ? launch<32, true>(a, n, nullptr) : launch<32, false>(a, n, nullptr);
 }

@@ -4,13 +4,10 @@
 // A value is a sign and a magnitude out of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (E2M1) times its block's scale:
 //   MXFP4  32 values share 2^(b - 127), one byte b (255 = NaN)
 //   NVFP4  16 values share an e4m3 number, one byte (0x7f = NaN)
-// Two orders of a quantised [rows][cols] matrix.  Both begin with the codes, row after row, value 2 i in the low half of byte i.
-// Behind them (on the next 256-byte boundary) stand the scales as words of four bytes, the four blocks of a row that
-// follow one another (128 values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there):
-//   rows     [word][row]: a product's activation tiles begin at any row, or gather their rows
-//   weights  [row / 128][word][row % 32][row / 32 % 4]: 512 bytes that go to tensor memory as they are
-#include <type_traits>
-
+// A quantised [rows][cols] matrix begins with the codes, row after row, value 2 i in the low half of byte i.  Behind them (on the
+// next 256-byte boundary) stand the scales as words of four bytes, the four blocks of a row that follow one another (128
+// values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there) and rows to one of 128:
+// [row / 128][word][row % 32][row / 32 % 4], 512 bytes of 128 rows that go to tensor memory as they are.
 namespace fp4 {
 
 constexpr uint32_t MX = 39u, NV = 40u;      // ggml type ids
@@ -19,15 +16,12 @@ constexpr uint32_t ROWS = 0u, WEIGHTS = 1u;
 __host__ __device__ constexpr uint32_t n_words(bool nv, uint32_t cols) { return (cols + 255u) / 256u * (nv ? 4u : 2u); }
 __host__ __device__ inline uint64_t up256(uint64_t v) { return (v + 255u) & ~(uint64_t)255u; }
 __host__ __device__ inline uint64_t code_bytes(uint64_t rows, uint32_t cols) { return up256(rows * (cols / 2u)); }
-__host__ __device__ inline uint64_t row_pitch(uint64_t rows) { return (rows + 3u) & ~(uint64_t)3u; }   // words of a line of the rows order
-inline uint64_t bytes(bool nv, uint32_t form, uint64_t rows, uint32_t cols) {
-    const uint64_t r = form == WEIGHTS ? (rows + 127u) / 128u * 128u : row_pitch(rows);
-    return code_bytes(rows, cols) + up256(r * n_words(nv, cols) * 4u);
+inline uint64_t bytes(bool nv, uint64_t rows, uint32_t cols) {
+    return code_bytes(rows, cols) + (rows + 127u) / 128u * n_words(nv, cols) * 512u;
 }
 // Byte offset, from the scales' beginning, of word w of a row.
-template <bool WF> __device__ __forceinline__ uint64_t word_at(uint64_t row, uint32_t w, uint32_t words, uint64_t pitch) {
-    if (WF) return ((row >> 7) * words + w) * 512u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u;
-    return (w * pitch + row) * 4u;
+__device__ __forceinline__ uint64_t word_at(uint64_t row, uint32_t w, uint32_t words) {
+    return ((row >> 7) * words + w) * 512u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u;
 }
 
 // ---- arithmetic of the formats ----
@@ -129,7 +123,7 @@ struct QArgs {
     const float *x;        // the rows, or gate | up rows
     uint64_t ld;
     float mul;
-    uint64_t rows, pitch;
+    uint64_t rows;
     uint32_t cols, words;
     uint8_t *codes, *scales;
 };
@@ -184,9 +178,9 @@ template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uin
 }
 
 // A warp takes 256 values of a row at a time, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same
-// columns of eight rows that follow one another, whose scale words lie side by side in the rows order; U such pieces of a row are
+// columns of eight rows that follow one another; U such pieces of a row are
 // loaded before the first is quantised.
-template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
+template <bool NVF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
     constexpr int U = SWIGLU ? 1 : 2;
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -203,7 +197,7 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 2 : 4);
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 4 : 8);
         if ((lane & (NVF ? 7u : 15u)) == 0u)
-            *reinterpret_cast<uint32_t *>(a.scales + word_at<WF>(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words, a.pitch)) = w;
+            *reinterpret_cast<uint32_t *>(a.scales + word_at(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words)) = w;
     };
     const uint32_t step = gridDim.y * 256u;
     for (uint32_t c0 = blockIdx.y * 256u; c0 < a.cols; c0 += U * step) {
@@ -259,8 +253,7 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
 }
 
 // A quantised matrix as the values that it stands for: a warp 256 values of a row at a time.
-template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows,
-                                                                                      uint64_t pitch, uint32_t cols, uint32_t words, float *out, uint64_t ld) {
+template <bool NVF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint32_t cols, uint32_t words, float *out, uint64_t ld) {
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t row = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
@@ -272,7 +265,7 @@ template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) va
             const uint32_t c = c0 + h * 128u + lane * 4u;
             if (c >= cols) continue;
             const uint32_t b = c >> (NVF ? 4 : 5);
-            const float s = scale_value<NVF>(scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)]) * 0.5f;
+            const float s = scale_value<NVF>(scales[word_at(row, b >> 2, words) + (b & 3u)]) * 0.5f;
             const uint32_t q = *reinterpret_cast<const uint16_t *>(codes + row * (cols >> 1) + (c >> 1));
             const uint32_t m = prmt(MAG_LO, MAG_HI, q & 0x7777u);
             float v[4];
@@ -308,7 +301,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *
                 const uint32_t b = p / PER * 4u + j;
                 if (b < nb) sw |= (uint32_t)(scales ? scales[r * nb + b] : codes[(r * nb + b) * 17u]) << (8u * j);
             }
-            *reinterpret_cast<uint32_t *>(to + scale_off + word_at<true>(row, p / PER, words, 0)) = sw;
+            *reinterpret_cast<uint32_t *>(to + scale_off + word_at(row, p / PER, words)) = sw;
         }
         if (p * 32u >= cols) continue;
         uint32_t q[4] = {0, 0, 0, 0};
@@ -334,8 +327,8 @@ struct MArgs {
     const uint8_t *w;                    // codes of the first matrix; its scales w_off bytes behind
     uint64_t w_off, stride;
     uint32_t w_rows, cols, words;
-    const uint8_t *x, *xs;               // codes and scales of the activations (rows order)
-    uint64_t x_rows, x_pitch;
+    const uint8_t *x, *xs;               // codes and scales of the activations
+    uint64_t x_rows;
     const int32_t *rows, *bounds;        // row p of the result is row rows[p] (or p) of x; expert e has rows [bounds[e], bounds[e + 1])
     uint32_t n_expert;
     uint64_t total;
@@ -394,7 +387,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) few_k(const MArgs a) 
             uint32_t xs = 0;
             if (there) {
                 x = *reinterpret_cast<const uint4 *>(a.x + xr * (a.cols >> 1) + (c >> 1));
-                xs = *reinterpret_cast<const uint32_t *>(a.xs + (wd * a.x_pitch + xr) * 4u) >> sh;
+                xs = *reinterpret_cast<const uint32_t *>(a.xs + word_at(xr, wd, a.words)) >> sh;
             }
             const uint4 ws = *reinterpret_cast<const uint4 *>(w + a.w_off + ((uint64_t)(r0 >> 7) * a.words + wd) * 512u + (r0 & 31u) * 16u);
             const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, wsw[4] = {ws.x, ws.y, ws.z, ws.w};
@@ -447,31 +440,25 @@ bool shape(uint32_t type, uint64_t rows, uint64_t cols) {
 }
 bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1u)) == 0; }
 
-template <bool SWIGLU>
-bool quantize(uint32_t type, uint32_t form, const float *x, uint64_t ld, float mul, uint64_t rows, uint64_t cols, void *q) {
+template <bool SWIGLU> bool quantize(uint32_t type, const float *x, uint64_t ld, float mul, uint64_t rows, uint64_t cols, void *q) {
     QArgs a;
     a.x = x;
     a.ld = ld;
     a.mul = mul;
     a.rows = rows;
-    a.pitch = row_pitch(rows);
     a.cols = (uint32_t)cols;
     a.words = n_words(type == NV, a.cols);
     a.codes = (uint8_t *)q;
     a.scales = a.codes + code_bytes(rows, a.cols);
-    const bool vec = aligned(x, 16) && ld % 4u == 0;
     OnDevice dev;
     // a row's pieces of 256 values to one warp while there are rows enough for all SMs
     const uint32_t groups = (uint32_t)((rows + 7u) / 8u), pieces = (a.cols + 255u) / 256u;
     const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
     const dim3 grid(groups, pieces < want ? pieces : want);
     auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, a); };
-    auto pick = [&](auto nv, auto wf) {
-        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
-        vec ? go(quantize_k<N, W, SWIGLU, true>) : go(quantize_k<N, W, SWIGLU, false>);
-    };
-    if (SWIGLU || form == ROWS) type == NV ? pick(std::true_type(), std::false_type()) : pick(std::false_type(), std::false_type());
-    else type == NV ? pick(std::true_type(), std::bool_constant<!SWIGLU>()) : pick(std::false_type(), std::bool_constant<!SWIGLU>());
+    const bool vec = aligned(x, 16) && ld % 4u == 0;
+    if (type == NV) vec ? go(quantize_k<true, SWIGLU, true>) : go(quantize_k<true, SWIGLU, false>);
+    else vec ? go(quantize_k<false, SWIGLU, true>) : go(quantize_k<false, SWIGLU, false>);
     g_q4b_launches++;
     return q4b_launch_ok("fp4 quantize");
 }
@@ -491,14 +478,14 @@ bool product(uint32_t type, MArgs &a) {
 }  // namespace fp4
 
 extern "C" uint64_t q4_cuda_fp4_bytes(uint32_t type, uint32_t form, uint64_t rows, uint64_t cols) {
-    return fp4::shape(type, rows, cols) && form <= fp4::WEIGHTS ? fp4::bytes(type == fp4::NV, form, rows, (uint32_t)cols) : 0u;
+    return fp4::shape(type, rows, cols) && form <= fp4::WEIGHTS ? fp4::bytes(type == fp4::NV, rows, (uint32_t)cols) : 0u;
 }
 
 extern "C" bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uint8_t *d_scales, uint64_t rows, uint64_t cols, uint64_t n_mat,
                                 void *d_w, uint64_t stride) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, cols) || !d_codes || !d_w || !n_mat || n_mat > 65535u || !aligned(d_w, 16) || stride % 16u ||
-        (n_mat > 1u && stride < bytes(type == NV, WEIGHTS, rows, (uint32_t)cols)) || (type == NV && !d_scales))
+        (n_mat > 1u && stride < bytes(type == NV, rows, (uint32_t)cols)) || (type == NV && !d_scales))
         return false;
     OnDevice dev;
     const uint32_t words = n_words(type == NV, (uint32_t)cols);
@@ -517,13 +504,13 @@ extern "C" bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uin
 extern "C" bool q4_cuda_fp4_quantize(uint32_t type, uint32_t form, const float *d_x, uint64_t ld_x, float mul, uint64_t rows, uint64_t cols, void *d_q) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, cols) || form > WEIGHTS || !d_x || !d_q || ld_x < cols || !aligned(d_x, 4) || !aligned(d_q, 16)) return false;
-    return quantize<false>(type, form, d_x, ld_x, mul, rows, cols, d_q);
+    return quantize<false>(type, d_x, ld_x, mul, rows, cols, d_q);
 }
 
 extern "C" bool q4_cuda_fp4_swiglu_quantize(uint32_t type, const float *d_gu, uint64_t ld_gu, float mul, uint64_t rows, uint64_t n_ff, void *d_hq) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, n_ff) || !d_gu || !d_hq || ld_gu < 2u * n_ff || !aligned(d_gu, 4) || !aligned(d_hq, 16)) return false;
-    return quantize<true>(type, ROWS, d_gu, ld_gu, mul, rows, n_ff, d_hq);
+    return quantize<true>(type, d_gu, ld_gu, mul, rows, n_ff, d_hq);
 }
 
 extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q, uint64_t rows, uint64_t cols, float *d_out, uint64_t ld_out) {
@@ -531,17 +518,13 @@ extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q
     if (!g_q4b.ok || !shape(type, rows, cols) || form > WEIGHTS || !d_q || !d_out || ld_out < cols || !aligned(d_q, 16) || !aligned(d_out, 4)) return false;
     OnDevice dev;
     const uint8_t *codes = (const uint8_t *)d_q, *scales = codes + code_bytes(rows, (uint32_t)cols);
-    const uint64_t pitch = row_pitch(rows);
     const uint32_t c = (uint32_t)cols, words = n_words(type == NV, c), groups = (uint32_t)((rows + 7u) / 8u), pieces = (c + 255u) / 256u;
     const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
     const dim3 grid(groups, pieces < want ? pieces : want);
-    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, pitch, c, words, d_out, ld_out); };
-    auto pick = [&](auto nv, auto wf) {
-        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
-        aligned(d_out, 16) && ld_out % 4u == 0 ? go(values_k<N, W, true>) : go(values_k<N, W, false>);
-    };
-    if (form == WEIGHTS) type == NV ? pick(std::true_type(), std::true_type()) : pick(std::false_type(), std::true_type());
-    else type == NV ? pick(std::true_type(), std::false_type()) : pick(std::false_type(), std::false_type());
+    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, c, words, d_out, ld_out); };
+    const bool vec = aligned(d_out, 16) && ld_out % 4u == 0;
+    if (type == NV) vec ? go(values_k<true, true>) : go(values_k<true, false>);
+    else vec ? go(values_k<false, true>) : go(values_k<false, false>);
     g_q4b_launches++;
     return q4b_launch_ok("fp4 values");
 }
@@ -561,7 +544,6 @@ extern "C" bool q4_cuda_fp4_mul(uint32_t type, const void *d_w, uint64_t w_rows,
     a.x = (const uint8_t *)d_xq;
     a.xs = a.x + code_bytes(rows, a.cols);
     a.x_rows = a.total = rows;
-    a.x_pitch = row_pitch(rows);
     a.n_expert = 1;
     a.scale = scale;
     a.dst = d_y;
@@ -576,7 +558,7 @@ extern "C" bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_ro
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, w_rows, w_cols) || !shape(type, xq_rows, w_cols) || !d_w || !d_xq || !d_bounds || !d_dst || ld_dst < w_rows ||
         !n_expert || n_expert > 1024u || expert_stride_bytes % 16u ||
-        (n_expert > 1u && expert_stride_bytes < bytes(type == NV, WEIGHTS, w_rows, (uint32_t)w_cols)) || total_rows > 0x7fffffffull ||
+        (n_expert > 1u && expert_stride_bytes < bytes(type == NV, w_rows, (uint32_t)w_cols)) || total_rows > 0x7fffffffull ||
         (!d_rows && total_rows > xq_rows) || !aligned(d_w, 16) || !aligned(d_xq, 16) || !aligned(d_dst, 4))
         return false;
     if (!total_rows) return true;
@@ -590,7 +572,6 @@ extern "C" bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_ro
     a.x = (const uint8_t *)d_xq;
     a.xs = a.x + code_bytes(xq_rows, a.cols);
     a.x_rows = xq_rows;
-    a.x_pitch = row_pitch(xq_rows);
     a.rows = d_rows;
     a.bounds = d_bounds;
     a.n_expert = n_expert;

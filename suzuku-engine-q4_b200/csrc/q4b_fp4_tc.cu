@@ -5,7 +5,7 @@
 // 128 x BN of the result (an expert's rows begin at any row; its last tile has fewer), and its warps have a task each:
 //   warp 0     copies: codes of x and W (TMA, 128-byte swizzle: 256 values of a row a stage), W's scales (bulk).  Gathered rows
 //              of x come by four (tile::gather4)
-//   warp 2     the scales of x: words of [word][row] that land where the tensor memory's layout wants them (cp.async)
+//   warps 2-3  of experts' rows, which begin anywhere: the scales of x, word by word (cp.async)
 //   warp 1     brings a stage's scales to tensor memory (tcgen05.cp) and issues its MMAs
 //   warps 4-7  read a finished accumulator, apply the factor, transpose 32 x 32 in shared memory and store whole lines, while
 //              the MMAs fill the other one
@@ -29,10 +29,10 @@ using mmqtc::tmem_ld_wait;
 constexpr uint32_t ERR_FP4 = 1u << 20;
 constexpr uint32_t KSTAGE = 256u;
 constexpr uint32_t MAX_EXPERTS = 1024u, MAX_MAP = 512u;
-constexpr uint32_t THREADS = 384u;
+constexpr uint32_t THREADS = 416u;
 
 struct TcSmem {
-    unsigned long long full[8], peer[8], empty[8], acc_full[2], acc_empty[2];
+    unsigned long long full[8], ready[8], empty[8], acc_full[2], acc_empty[2];
     uint32_t tmem, warp_sum[8];
     uint32_t first[MAX_EXPERTS + 1];       // tiles of rows before every expert
     int32_t row[MAX_EXPERTS + 1];          // its first row
@@ -119,7 +119,7 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
     q4b_pdl_wait();
     if (tid == 0) {
-        for (uint32_t i = 0; i < C::NS; i++) mbar_init(&s.full[i], 1 + 64), mbar_init(&s.peer[i], 1), mbar_init(&s.empty[i], 1);
+        for (uint32_t i = 0; i < C::NS; i++) mbar_init(&s.full[i], a.bounds ? 1 + 64 : 1), mbar_init(&s.ready[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
         for (uint32_t i = 0; i < 2u; i++) mbar_init(&s.acc_full[i], 1), mbar_init(&s.acc_empty[i], PAIR ? 16 : 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -227,8 +227,10 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
             const Tile tl = tile_of(t);
             const uint32_t n_box = a.rows ? 0u : ((uint32_t)tl.rows + 31u) / 32u;
             const uint32_t a0 = tl.n0 >> 7, blocks = (a.w_rows + 127u) >> 7, atoms = min(C::ATOMS, blocks - a0);
-            const uint32_t bytes = n_box * 4096u + C::B + atoms * C::WPS * 512u;
-            const uint8_t *ws = a.w + tl.e * a.stride + a.w_off + (uint64_t)a0 * a.words * 512u;
+            const bool xs_too = !a.bounds && tl.rows > 0;            // a dense product's tiles begin where a block of scales does
+            const uint32_t bytes = n_box * 4096u + C::B + (atoms + (xs_too ? 1u : 0u)) * C::WPS * 512u;
+            const uint8_t *const xs = a.xs + (uint64_t)((uint32_t)tl.m0 >> 7) * a.words * 512u;
+            const uint8_t *const ws = a.w + tl.e * a.stride + a.w_off + (uint64_t)a0 * a.words * 512u;
             for (uint32_t k = 0; k < n_ks; k++, it++) {
                 const uint32_t sl = it % C::NS;
                 uint8_t *st = ring + sl * C::STAGE;
@@ -240,52 +242,16 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                     for (uint32_t i = 0; i < atoms; i++)
                         bulk_load(smem_u32(st + C::A + C::B + C::SA + i * C::WPS * 512u), ws + ((uint64_t)i * a.words + k * C::WPS) * 512u, C::WPS * 512u,
                                   &s.full[sl]);
+                    if (xs_too) bulk_load(smem_u32(st + C::A + C::B), xs + (uint64_t)(k * C::WPS) * 512u, C::WPS * 512u, &s.full[sl]);
                     for (uint32_t i = 0; i < n_box; i++) tma_load_2d(st + i * 4096u, &maps.x, &s.full[sl], (int)(k * 128u), tl.m0 + (int)(i * 32u));
                 }
                 __syncwarp();
             }
         }
-    } else if (warp == 1 && rank == 0) {
-        // ---- scales to tensor memory, MMAs ----
-        if (elect_one()) {
-            const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((NVF ? 0u : 1u) << 23) | ((PAIR ? 2u : 1u) << 27);
-            const uint64_t d0 = smem_desc_sw128(smem_u32(ring));
-            uint32_t it = 0, n = 0;
-            for (uint32_t t = unit; t < all; t += units, n++) {
-                const uint32_t acc = n & 1u, n0 = (t % n_tiles) * BN;
-                if (n >= 2u) wait(&s.acc_empty[acc], (n / 2u - 1u) & 1u);
-                tc_fence_after();
-                for (uint32_t k = 0; k < n_ks; k++, it++) {
-                    const uint32_t sl = it % C::NS, at = sl * C::STAGE;
-                    wait(&s.full[sl], (it / C::NS) & 1u);
-                    if (PAIR) wait(&s.peer[sl], (it / C::NS) & 1u);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    tc_fence_after();
-                    const uint32_t sf = tmem + C::SF_AT + (it & 1u) * C::SF_COLS, sfb = sf + C::WPS * 4u;
-                    const uint32_t sa = smem_u32(ring) + at + C::A + C::B;
-#pragma unroll
-                    for (uint32_t w = 0; w < C::WPS; w++) scales_to_tmem<PAIR>(sf + w * 4u, sa + w * 512u);
-#pragma unroll
-                    for (uint32_t i = 0; i < C::ATOMS; i++)
-#pragma unroll
-                        for (uint32_t w = 0; w < C::WPS; w++)
-                            scales_to_tmem<PAIR>(sfb + (w * C::ATOMS + i) * 4u, sa + C::SA + (i * C::WPS + w) * 512u);
-                    const uint32_t left = a.cols - k * KSTAGE, n_mma = left >= KSTAGE ? 4u : (left + 63u) / 64u;
-                    const uint64_t da = d0 + (at >> 4), db = da + (C::A >> 4);
-                    for (uint32_t j = 0; j < n_mma; j++) {
-                        const uint32_t w = NVF ? j : j >> 1, id = NVF ? 0u : (j & 1u) * 2u;
-                        mma_fp4<NVF, PAIR>(tmem + acc * BN, da + j * 2u, db + j * 2u, idesc0 | (id << 4) | (id << 29), sf + w * 4u,
-                                           sfb + w * C::ATOMS * 4u + ((n0 & 127u) >> 5), (k | j) ? 1u : 0u);
-                    }
-                    if (PAIR) mmqtc::mma_commit2(&s.empty[sl]);
-                    else mma_commit(&s.empty[sl]);
-                }
-                if (PAIR) mmqtc::mma_commit2(&s.acc_full[acc]);
-                else mma_commit(&s.acc_full[acc]);
-            }
-        }
     } else if (warp == 1) {
-        // ---- the second CTA of a pair: tells the first one that a stage is there ----
+        // ---- a stage is there: its copies and the scales' are seen by this thread, made visible to the tensor cores and
+        // reported to the warp that issues the MMAs (of a pair, in the first CTA).  A barrier of its own and no fence there: what
+        // that thread does beside issuing is time in which the tensor cores idle ----
         if (elect_one()) {
             uint32_t it = 0;
             for (uint32_t t = unit; t < all; t += units)
@@ -294,15 +260,16 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     tc_fence_after();
                     tc_fence_before();
-                    mmqtc::mbar_arrive_cluster(mmqtc::leader_addr(&s.peer[it % C::NS]));
+                    if (PAIR) mmqtc::mbar_arrive_cluster(mmqtc::leader_addr(&s.ready[it % C::NS]));
+                    else mbar_arrive(&s.ready[it % C::NS]);
                 }
         }
     } else if (warp < 4u) {
-        // ---- the scales of x, and its codes where rows are gathered: 64 rows each.  A lane arrives when its copies have landed; who
+        // ---- experts' rows, which begin anywhere: the scales of x, and its codes where rows are gathered: 64 rows each.  A lane arrives when its copies have landed; who
         // has waited for all makes them visible to the tensor cores ----
         const uint32_t half = (warp & 1u) * 64u;
         uint32_t it = 0;
-        for (uint32_t t = unit; t < all; t += units) {
+        for (uint32_t t = a.bounds ? unit : all; t < all; t += units) {
             const Tile tl = tile_of(t);
             // lane l: scales of rows l and l + 32, sixteen bytes l % 8 of the codes of rows 4 i + l / 8
             const uint8_t *src[2];
@@ -315,7 +282,7 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                     x = (uint32_t)(a.rows ? a.rows[tl.m0 + r] : tl.m0 + r);
                     ok = x < (uint32_t)a.x_rows;
                 }
-                src[j] = a.xs + (ok ? (uint64_t)x : 0u) * 4u;
+                src[j] = a.xs + word_at(ok ? x : 0u, 0u, a.words);
                 size[j] = ok ? 4u : 0u;
                 if (a.rows) {
 #pragma unroll
@@ -331,7 +298,7 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
 #pragma unroll
                     for (uint32_t j = 0; j < 2u; j++)
                         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + w * 512u + j * 4u),
-                                     "l"(src[j] + (uint64_t)(k * C::WPS + w) * a.x_pitch * 4u), "r"(size[j])
+                                     "l"(src[j] + (uint64_t)(k * C::WPS + w) * 512u), "r"(size[j])
                                      : "memory");
                 if (a.rows) {
                     const uint32_t c = k * 128u + (lane & 7u) * 16u;
@@ -346,6 +313,47 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                     }
                 }
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full[sl])) : "memory");
+            }
+        }
+    } else if (warp == 12u) {
+        // ---- scales to tensor memory, MMAs ----
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc0 = (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((NVF ? 0u : 1u) << 23) | ((PAIR ? 2u : 1u) << 27);
+            const uint64_t d0 = smem_desc_sw128(smem_u32(ring));
+            uint32_t n = 0, sl = 0, par = 0, odd = 0;       // tiles; the stage's slot, its parity, its half of the scales' columns
+            for (uint32_t t = unit; t < all; t += units, n++) {
+                const uint32_t acc = n & 1u, n0 = (t % n_tiles) * BN;
+                if (n >= 2u) wait(&s.acc_empty[acc], (n / 2u - 1u) & 1u);
+                tc_fence_after();
+                for (uint32_t k = 0; k < n_ks; k++) {
+                    const uint32_t at = sl * C::STAGE;
+                    wait(&s.ready[sl], par);
+                    tc_fence_after();
+                    const uint32_t sf = tmem + C::SF_AT + odd * C::SF_COLS, sfb = sf + C::WPS * 4u;
+                    const uint32_t sa = smem_u32(ring) + at + C::A + C::B;
+#pragma unroll
+                    for (uint32_t w = 0; w < C::WPS; w++) scales_to_tmem<PAIR>(sf + w * 4u, sa + w * 512u);
+#pragma unroll
+                    for (uint32_t i = 0; i < C::ATOMS; i++)
+#pragma unroll
+                        for (uint32_t w = 0; w < C::WPS; w++)
+                            scales_to_tmem<PAIR>(sfb + (w * C::ATOMS + i) * 4u, sa + C::SA + (i * C::WPS + w) * 512u);
+                    const uint32_t left = a.cols - k * KSTAGE, n_mma = left >= KSTAGE ? 4u : (left + 63u) / 64u;
+                    const uint64_t da = d0 + (at >> 4), db = da + (C::A >> 4);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        if (j >= n_mma) break;
+                        const uint32_t w = NVF ? j : j >> 1, id = NVF ? 0u : (j & 1u) * 2u;
+                        mma_fp4<NVF, PAIR>(tmem + acc * BN, da + j * 2u, db + j * 2u, idesc0 | (id << 4) | (id << 29), sf + w * 4u,
+                                           sfb + w * C::ATOMS * 4u + ((n0 & 127u) >> 5), (k | j) ? 1u : 0u);
+                    }
+                    if (PAIR) mmqtc::mma_commit2(&s.empty[sl]);
+                    else mma_commit(&s.empty[sl]);
+                    odd ^= 1u;
+                    if (++sl == C::NS) sl = 0, par ^= 1u;
+                }
+                if (PAIR) mmqtc::mma_commit2(&s.acc_full[acc]);
+                else mma_commit(&s.acc_full[acc]);
             }
         }
     } else {
@@ -374,11 +382,14 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                 tmem_ld_wait();
 #pragma unroll
                 for (uint32_t i = 0; i < 32u; i++) v[i] = there ? v[i] * f : 0.f;
-                if (mine <= 4 && vec && col + 32u <= a.w_rows) {       // few rows: each from its lane
+                if (mine < 32 && vec && col + 32u <= a.w_rows) {       // fewer rows: each from its lane, in whole sectors
                     if ((int32_t)lane < mine) {
-                        float4 *o = reinterpret_cast<float4 *>(base + (uint64_t)lane * a.ld + col);
+                        float *o = base + (uint64_t)lane * a.ld + col;
 #pragma unroll
-                        for (uint32_t i = 0; i < 8u; i++) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        for (uint32_t i = 0; i < 4u; i++)
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + 8 * i), "f"(v[8 * i]), "f"(v[8 * i + 1]),
+                                         "f"(v[8 * i + 2]), "f"(v[8 * i + 3]), "f"(v[8 * i + 4]), "f"(v[8 * i + 5]), "f"(v[8 * i + 6]), "f"(v[8 * i + 7])
+                                         : "memory");
                     }
                     continue;
                 }
@@ -403,20 +414,11 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                     continue;
                 }
                 __syncwarp();
-                if (vec && col + 32u <= a.w_rows) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) {
-                        const uint32_t r = i * 4u + (lane >> 3), c = lane & 7u;
-                        const float4 o = *reinterpret_cast<const float4 *>(buf + r * 128u + ((c ^ (r & 7u)) << 4));
-                        if ((int32_t)r < mine) *reinterpret_cast<float4 *>(base + (uint64_t)r * a.ld + col + 4u * c) = o;
-                    }
-                } else {
-                    const bool in = col + lane < a.w_rows;
+                const bool in = col + lane < a.w_rows;
 #pragma unroll 8
-                    for (uint32_t r = 0; r < 32u; r++) {
-                        const float o = *reinterpret_cast<const float *>(buf + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u);
-                        if (in && (int32_t)r < mine) base[(uint64_t)r * a.ld + col + lane] = o;
-                    }
+                for (uint32_t r = 0; r < 32u; r++) {
+                    const float o = *reinterpret_cast<const float *>(buf + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u);
+                    if (in && (int32_t)r < mine) base[(uint64_t)r * a.ld + col + lane] = o;
                 }
                 __syncwarp();
             }
@@ -454,7 +456,7 @@ template <bool NVF, uint32_t BN, bool PAIR> bool tc_launch(const MArgs &a, uint6
     const cuuint32_t xb[2] = {128, 32}, wb[3] = {128, C::BH, 1};
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     if (!encode(&maps.x, u8, 2, a.x, xd, xs, xb) || !encode(&maps.w, u8, 3, a.w, wd, ws, wb)) return false;
-    const bool vec = aligned(a.dst, 16) && a.ld % 4u == 0 && a.ld * 4u < (1ull << 40);      // whole lines of the result at a time
+    const bool vec = aligned(a.dst, 32) && a.ld % 8u == 0 && a.ld * 4u < (1ull << 40);      // whole sectors of the result
     maps.y = maps.x;
     const cuuint64_t yd[2] = {a.w_rows, a.total}, ys[1] = {a.ld * 4u};
     const cuuint32_t yb[2] = {32, 32};
@@ -500,6 +502,7 @@ bool tc_product(bool nv, const MArgs &a) {
     if (!g_tc_ready) return false;
     const uint64_t m_tiles = a.bounds ? (a.total < a.n_expert ? a.total : a.n_expert) + a.total / 128u : (a.total + 127u) / 128u;
     if (m_tiles * ((a.w_rows + 63u) / 64u) > 0x7fffffffull) return false;
+    if (getenv("Q4B_FP4_TILE")) { uint32_t v = atoi(getenv("Q4B_FP4_TILE")); if (v >= 1000) return tc_go<192, true>(nv, a, (a.bounds ? (a.total < a.n_expert ? a.total : a.n_expert) : 1) + a.total / 256u); return v == 192u ? tc_go<192, false>(nv, a, m_tiles) : v == 128u ? tc_go<128, false>(nv, a, m_tiles) : tc_go<64, false>(nv, a, m_tiles); }
     const uint64_t pairs = (a.total + 255u) / 256u;
     if (!a.bounds && pairs * ((a.w_rows + 191u) / 192u) >= 4u * (uint64_t)g_q4b.n_sm) return tc_go<192, true>(nv, a, pairs);
     uint64_t best = ~0ull;
