@@ -631,19 +631,18 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  *   Q4_T_NVFP4  16 values share an e4m3 number; byte 0x7f = NaN.  A factor for a whole matrix, where there is one, is
  *               the caller's and goes into the products' scale
  * Quantising v = x * mul (rounded to fp32): MXFP4 takes the power of two floor(log2 max|v|) - 2 (-127 at least), NVFP4 the
- * e4m3 number nearest to max|v| / 6 (448 at most; a block that this rounds to 0 is zeros); codes are the nearest, ties to even, 6
- * for all beyond it.  A block with an infinity or a NaN becomes NaN.
+ * e4m3 number nearest to max|v| times fp32's 1/6 (448 at most; a block that this rounds to 0 is zeros); codes are the nearest,
+ * ties to even, 6 for all beyond it.  A block with an infinity or a NaN becomes NaN.
  * cols: a multiple of 32, at most 65536; any number of rows below 2^31.  A quantised matrix is an opaque
- * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned.  form says what it is for:
+ * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned, in one of two forms:
  *   Q4_FP4_ROWS     activations: what the products take as d_xq
  *   Q4_FP4_WEIGHTS  weights: what they take as d_w; the matrices of several experts stand a stride apart
- * (the bytes of both are in the same order, so that a product of two activations is one call, too)
  *   put              n_mat matrices of a checkpoint -> weights at d_w + i * stride.  d_codes [n_mat][rows][cols / 2], value 2 i
  *                    in the low half of byte i; d_scales [n_mat][rows][cols / 32 or 16].  d_scales == NULL (MXFP4): d_codes
  *                    holds ggml blocks of 17 bytes, the scale first, values j and j + 16 in the halves of byte j
  *   quantize         fp32 rows, ld_x floats apart, -> either form
- *   swiglu_quantize  silu(gu[r][k]) * gu[r][n_ff + k] * mul -> rows form.  The codes are those of the exact values (one
- *                    that fp32 leaves next to a border is computed again in 64 bits)
+ *   swiglu_quantize  silu(gu[r][k]) * gu[r][n_ff + k] * mul -> rows form.  Scales and codes are those of the exact
+ *                    values (and of max / 6; one that fp32 leaves next to a border is computed again in 64 bits)
  *   values           either form -> the fp32 values that it stands for
  *   mul              d_y[t][r] = scale * W[r] . x[t], ld_y floats apart; rows is the one that d_xq was made with
  *   mul_id           row p of d_dst, for expert e's p in [bounds[e], bounds[e + 1]) (device int32, n_expert + 1 entries, ascending;

@@ -6,8 +6,11 @@
 //   NVFP4  16 values share an e4m3 number, one byte (0x7f = NaN)
 // A quantised [rows][cols] matrix begins with the codes, row after row, value 2 i in the low half of byte i.  Behind them (on the
 // next 256-byte boundary) stand the scales as words of four bytes, the four blocks of a row that follow one another (128
-// values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there) and rows to one of 128:
-// [row / 128][word][row % 32][row / 32 % 4], 512 bytes of 128 rows that go to tensor memory as they are.
+// values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there):
+//   rows     [word][row]: a product's tiles of activations begin at any row, or gather their rows
+//   weights  [row / 128][word][row % 32][row / 32 % 4]: 512 bytes that go to tensor memory as they are
+#include <type_traits>
+
 namespace fp4 {
 
 constexpr uint32_t MX = 39u, NV = 40u;      // ggml type ids
@@ -16,12 +19,14 @@ constexpr uint32_t ROWS = 0u, WEIGHTS = 1u;
 __host__ __device__ constexpr uint32_t n_words(bool nv, uint32_t cols) { return (cols + 255u) / 256u * (nv ? 4u : 2u); }
 __host__ __device__ inline uint64_t up256(uint64_t v) { return (v + 255u) & ~(uint64_t)255u; }
 __host__ __device__ inline uint64_t code_bytes(uint64_t rows, uint32_t cols) { return up256(rows * (cols / 2u)); }
-inline uint64_t bytes(bool nv, uint64_t rows, uint32_t cols) {
-    return code_bytes(rows, cols) + (rows + 127u) / 128u * n_words(nv, cols) * 512u;
+__host__ __device__ inline uint64_t row_pitch(uint64_t rows) { return (rows + 3u) & ~(uint64_t)3u; }   // words of a line of the rows order
+inline uint64_t bytes(bool nv, uint32_t form, uint64_t rows, uint32_t cols) {
+    return code_bytes(rows, cols) + up256((form == WEIGHTS ? (rows + 127u) / 128u * 128u : row_pitch(rows)) * n_words(nv, cols) * 4u);
 }
 // Byte offset, from the scales' beginning, of word w of a row.
-__device__ __forceinline__ uint64_t word_at(uint64_t row, uint32_t w, uint32_t words) {
-    return ((row >> 7) * words + w) * 512u + (row & 31u) * 16u + ((row >> 5) & 3u) * 4u;
+template <bool WF> __device__ __forceinline__ uint64_t word_at(uint64_t row, uint32_t w, uint32_t words, uint64_t pitch) {
+    if (WF) return ((row >> 7) * words + w) * 512u + ((uint32_t)row & 31u) * 16u + ((uint32_t)(row >> 5) & 3u) * 4u;
+    return (w * pitch + row) * 4u;
 }
 
 // ---- arithmetic of the formats ----
@@ -63,11 +68,10 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
 template <bool NVF> __device__ __forceinline__ float scale_value(uint32_t b) { return NVF ? e4m3_value(b) : e8m0_value(b); }
 
 // The scale byte of a block whose largest magnitude is a.  MXFP4: the power of two that brings a into [4, 8); NVFP4: a sixth
-// of a, rounded to e4m3.  (A quotient by 6 that is not on a border between two e4m3 numbers is not rounded onto one: such
-// a border has five bits and six times it is an fp32 number, so a differs from that by a step of its own at least.)
+// of a (its product with fp32's 1/6), rounded to e4m3.
 template <bool NVF> __device__ __forceinline__ uint32_t scale_byte(float a) {
     if (!(a <= 3.402823466e38f)) return NVF ? 0x7fu : 255u;
-    if (NVF) return e4m3_nearest(__fdiv_rn(a, 6.f));
+    if (NVF) return e4m3_nearest(a * (1.f / 6.f));
     const int e = (int)(__float_as_uint(a) >> 23) - 2;      // 127 + floor(log2 a) - 2 for a normal a, at most 252
     return (uint32_t)max(e, 0);
 }
@@ -79,7 +83,8 @@ template <bool NVF> __device__ __forceinline__ float inverse(uint32_t sb) {
 }
 // Eight values of a block with that scale to codes.  MXFP4: the product with the inverse power of two is exact.  NVFP4: the quotient
 // by the scale is rounded correctly (Markstein 1990: a product with the rounded inverse, corrected once by its exact remainder), and then
-// falls on a border between two codes only where the exact one does (as above: the scale has four bits, a border three).
+// falls on a border between two codes only where the exact one does: the scale has four bits and a border three, so a border's value
+// is an fp32 number, and one that is not on it is a step of fp32 away at least.
 template <bool NVF> __device__ __forceinline__ uint32_t codes8(const float *v, uint32_t sb) {
     const float inv = inverse<NVF>(sb);
     float t[8];
@@ -123,7 +128,7 @@ struct QArgs {
     const float *x;        // the rows, or gate | up rows
     uint64_t ld;
     float mul;
-    uint64_t rows;
+    uint64_t rows, pitch;
     uint32_t cols, words;
     uint8_t *codes, *scales;
 };
@@ -180,7 +185,7 @@ template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uin
 // A warp takes 256 values of a row at a time, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same
 // columns of eight rows that follow one another; U such pieces of a row are
 // loaded before the first is quantised.
-template <bool NVF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
+template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
     constexpr int U = SWIGLU ? 1 : 2;
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
@@ -197,7 +202,7 @@ template <bool NVF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 2 : 4);
         w |= __shfl_xor_sync(0xffffffffu, w, NVF ? 4 : 8);
         if ((lane & (NVF ? 7u : 15u)) == 0u)
-            *reinterpret_cast<uint32_t *>(a.scales + word_at(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words)) = w;
+            *reinterpret_cast<uint32_t *>(a.scales + word_at<WF>(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words, a.pitch)) = w;
     };
     const uint32_t step = gridDim.y * 256u;
     for (uint32_t c0 = blockIdx.y * 256u; c0 < a.cols; c0 += U * step) {
@@ -253,7 +258,8 @@ template <bool NVF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256
 }
 
 // A quantised matrix as the values that it stands for: a warp 256 values of a row at a time.
-template <bool NVF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint32_t cols, uint32_t words, float *out, uint64_t ld) {
+template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t pitch, uint32_t cols, uint32_t words,
+                                                                                      float *out, uint64_t ld) {
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t row = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
@@ -265,7 +271,7 @@ template <bool NVF, bool VEC> __global__ void __launch_bounds__(256) values_k(co
             const uint32_t c = c0 + h * 128u + lane * 4u;
             if (c >= cols) continue;
             const uint32_t b = c >> (NVF ? 4 : 5);
-            const float s = scale_value<NVF>(scales[word_at(row, b >> 2, words) + (b & 3u)]) * 0.5f;
+            const float s = scale_value<NVF>(scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)]) * 0.5f;
             const uint32_t q = *reinterpret_cast<const uint16_t *>(codes + row * (cols >> 1) + (c >> 1));
             const uint32_t m = prmt(MAG_LO, MAG_HI, q & 0x7777u);
             float v[4];
@@ -301,7 +307,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *
                 const uint32_t b = p / PER * 4u + j;
                 if (b < nb) sw |= (uint32_t)(scales ? scales[r * nb + b] : codes[(r * nb + b) * 17u]) << (8u * j);
             }
-            *reinterpret_cast<uint32_t *>(to + scale_off + word_at(row, p / PER, words)) = sw;
+            *reinterpret_cast<uint32_t *>(to + scale_off + word_at<true>(row, p / PER, words, 0)) = sw;
         }
         if (p * 32u >= cols) continue;
         uint32_t q[4] = {0, 0, 0, 0};
@@ -328,7 +334,7 @@ struct MArgs {
     uint64_t w_off, stride;
     uint32_t w_rows, cols, words;
     const uint8_t *x, *xs;               // codes and scales of the activations
-    uint64_t x_rows;
+    uint64_t x_rows, x_pitch;
     const int32_t *rows, *bounds;        // row p of the result is row rows[p] (or p) of x; expert e has rows [bounds[e], bounds[e + 1])
     uint32_t n_expert;
     uint64_t total;
@@ -359,12 +365,17 @@ template <bool NVF> __device__ __forceinline__ float scaled(int d, uint32_t sw, 
 }
 
 // One row of the result a CTA row (blockIdx.y), a warp four weight rows 32 apart (their scale words are 16 bytes).  A lane takes 32
-// values, whose activations it decodes once for the four rows.
+// values at a time, whose activations it decodes once for the four rows.  Bound by the latency of the weights' reads: a CTA asks for
+// its weights (into the L2) before it waits for the kernel ahead, which quantises the activations, and a lane has the loads of
+// 2048 columns under way at a time.
 template <bool NVF> __global__ void __launch_bounds__(256) few_k(const MArgs a) {
-    q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t set = blockIdx.x * 8u + warp;                       // rows of tile set / 32, set % 32 + 32 j
     const uint32_t r0 = (set >> 5) * 128u + (set & 31u);
+    if (!a.bounds && r0 < a.w_rows)
+        for (uint32_t j = 0; j < 4u && r0 + 32u * j < a.w_rows; j++)
+            for (uint32_t c = lane * 256u; c < a.cols; c += 8192u) q4b_l2_prefetch(a.w + (uint64_t)(r0 + 32u * j) * (a.cols >> 1) + (c >> 1));
+    q4b_pdl_wait();
     if (r0 >= a.w_rows) return;
     for (uint64_t p = blockIdx.y; p < a.total; p += gridDim.y) {
         uint32_t e = 0;
@@ -381,36 +392,48 @@ template <bool NVF> __global__ void __launch_bounds__(256) few_k(const MArgs a) 
         const bool there = xr < a.x_rows;       // a row that is not there gives zeros
         const uint8_t *w = a.w + e * a.stride;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t c = lane * 32u; c < a.cols; c += 1024u) {
-            const uint32_t wd = c >> (NVF ? 6 : 7), sh = NVF ? (c >> 1) & 16u : (c >> 2) & 24u;    // the first of its scales in that word
-            uint4 x = make_uint4(0, 0, 0, 0);
-            uint32_t xs = 0;
-            if (there) {
-                x = *reinterpret_cast<const uint4 *>(a.x + xr * (a.cols >> 1) + (c >> 1));
-                xs = *reinterpret_cast<const uint32_t *>(a.xs + word_at(xr, wd, a.words)) >> sh;
-            }
-            const uint4 ws = *reinterpret_cast<const uint4 *>(w + a.w_off + ((uint64_t)(r0 >> 7) * a.words + wd) * 512u + (r0 & 31u) * 16u);
-            const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, wsw[4] = {ws.x, ws.y, ws.z, ws.w};
-            uint32_t m[8];
+        for (uint32_t c0 = lane * 32u; c0 < a.cols; c0 += 2048u) {
+            uint4 x[2], q[2][4], ws[2];
+            uint32_t xs[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                m[2 * i] = prmt(MAG_LO, MAG_HI, xw[i] & 0x7777u), m[2 * i + 1] = prmt(MAG_LO, MAG_HI, (xw[i] >> 16) & 0x7777u);
+            for (int h = 0; h < 2; h++) {
+                const uint32_t c = c0 + 1024u * h, wd = c >> (NVF ? 6 : 7);
+                x[h] = make_uint4(0, 0, 0, 0), xs[h] = 0;
+                if (c >= a.cols) continue;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t r = r0 + 32u * j;
-                if (r >= a.w_rows) break;
-                const uint4 q = *reinterpret_cast<const uint4 *>(w + (uint64_t)r * (a.cols >> 1) + (c >> 1));
-                const uint32_t qw[4] = {q.x, q.y, q.z, q.w}, s = wsw[j] >> sh;
-                int pos = 0, neg = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    dot8(qw[i], xw[i] & 0x88888888u, m[2 * i], m[2 * i + 1], pos, neg);
-                    if (NVF && i == 1) {
-                        acc[j] += scaled<true>(pos - neg, s & 0xffu, xs & 0xffu);
-                        pos = neg = 0;
-                    }
+                for (int j = 0; j < 4; j++)
+                    if (r0 + 32u * j < a.w_rows) q[h][j] = *reinterpret_cast<const uint4 *>(w + (uint64_t)(r0 + 32u * j) * (a.cols >> 1) + (c >> 1));
+                ws[h] = *reinterpret_cast<const uint4 *>(w + a.w_off + word_at<true>(r0, wd, a.words, 0));
+                if (there) {
+                    x[h] = *reinterpret_cast<const uint4 *>(a.x + xr * (a.cols >> 1) + (c >> 1));
+                    xs[h] = *reinterpret_cast<const uint32_t *>(a.xs + word_at<false>(xr, wd, a.words, a.x_pitch));
                 }
-                acc[j] += scaled<NVF>(pos - neg, NVF ? (s >> 8) & 0xffu : s & 0xffu, NVF ? (xs >> 8) & 0xffu : xs & 0xffu);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t c = c0 + 1024u * h;
+                if (c >= a.cols) break;
+                const uint32_t sh = NVF ? (c >> 1) & 16u : (c >> 2) & 24u;       // the first of the lane's scales in its word
+                const uint32_t xw[4] = {x[h].x, x[h].y, x[h].z, x[h].w}, wsw[4] = {ws[h].x, ws[h].y, ws[h].z, ws[h].w}, xsw = xs[h] >> sh;
+                uint32_t m[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    m[2 * i] = prmt(MAG_LO, MAG_HI, xw[i] & 0x7777u), m[2 * i + 1] = prmt(MAG_LO, MAG_HI, (xw[i] >> 16) & 0x7777u);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (r0 + 32u * j >= a.w_rows) break;
+                    const uint32_t qw[4] = {q[h][j].x, q[h][j].y, q[h][j].z, q[h][j].w}, s = wsw[j] >> sh;
+                    int pos = 0, neg = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        dot8(qw[i], xw[i] & 0x88888888u, m[2 * i], m[2 * i + 1], pos, neg);
+                        if (NVF && i == 1) {
+                            acc[j] += scaled<true>(pos - neg, s & 0xffu, xsw & 0xffu);
+                            pos = neg = 0;
+                        }
+                    }
+                    acc[j] += scaled<NVF>(pos - neg, NVF ? (s >> 8) & 0xffu : s & 0xffu, NVF ? (xsw >> 8) & 0xffu : xsw & 0xffu);
+                }
             }
         }
         const float f = a.each ? a.scale * a.each[e] : a.scale;
@@ -440,12 +463,13 @@ bool shape(uint32_t type, uint64_t rows, uint64_t cols) {
 }
 bool aligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1u)) == 0; }
 
-template <bool SWIGLU> bool quantize(uint32_t type, const float *x, uint64_t ld, float mul, uint64_t rows, uint64_t cols, void *q) {
+template <bool SWIGLU> bool quantize(uint32_t type, uint32_t form, const float *x, uint64_t ld, float mul, uint64_t rows, uint64_t cols, void *q) {
     QArgs a;
     a.x = x;
     a.ld = ld;
     a.mul = mul;
     a.rows = rows;
+    a.pitch = row_pitch(rows);
     a.cols = (uint32_t)cols;
     a.words = n_words(type == NV, a.cols);
     a.codes = (uint8_t *)q;
@@ -457,17 +481,28 @@ template <bool SWIGLU> bool quantize(uint32_t type, const float *x, uint64_t ld,
     const dim3 grid(groups, pieces < want ? pieces : want);
     auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, a); };
     const bool vec = aligned(x, 16) && ld % 4u == 0;
-    if (type == NV) vec ? go(quantize_k<true, SWIGLU, true>) : go(quantize_k<true, SWIGLU, false>);
-    else vec ? go(quantize_k<false, SWIGLU, true>) : go(quantize_k<false, SWIGLU, false>);
+    auto pick = [&](auto nv, auto wf) {
+        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
+        vec ? go(quantize_k<N, W, SWIGLU, true>) : go(quantize_k<N, W, SWIGLU, false>);
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    using weights = std::bool_constant<!SWIGLU>;
+    if (form == ROWS) type == NV ? pick(yes(), no()) : pick(no(), no());
+    else type == NV ? pick(yes(), weights()) : pick(no(), weights());
     g_q4b_launches++;
     return q4b_launch_ok("fp4 quantize");
 }
 
 bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
 
+// Few rows on the CUDA cores while their work is that of two CTAs of 2048 columns an SM, else on the tensor cores.  us with the
+// quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 7.0, 2 rows 6.5 / 7.0, 3 rows 9.1 / 7.0;
+// 8192 x 2560 1 row 8.5 / 8.0; 1024 x 1024 1 row 3.9 / 5.3, 8 rows 4.4 / 5.4.
 bool product(uint32_t type, MArgs &a) {
     OnDevice dev;
-    if (a.total > 4u) return tc_product(type == NV, a);
+    const uint64_t ctas = a.total * ((a.w_rows + 127u) / 128u * 4u);
+    if (ctas * a.cols > 2u * (uint64_t)g_q4b.n_sm * 2048u) return tc_product(type == NV, a);
     const dim3 grid((a.w_rows + 127u) / 128u * 4u, (unsigned)(a.total < 65535u ? a.total : 65535u));
     if (type == NV) q4b_launch(few_k<true>, grid, dim3(256), 0, g_q4b.stream, a);
     else q4b_launch(few_k<false>, grid, dim3(256), 0, g_q4b.stream, a);
@@ -478,14 +513,14 @@ bool product(uint32_t type, MArgs &a) {
 }  // namespace fp4
 
 extern "C" uint64_t q4_cuda_fp4_bytes(uint32_t type, uint32_t form, uint64_t rows, uint64_t cols) {
-    return fp4::shape(type, rows, cols) && form <= fp4::WEIGHTS ? fp4::bytes(type == fp4::NV, rows, (uint32_t)cols) : 0u;
+    return fp4::shape(type, rows, cols) && form <= fp4::WEIGHTS ? fp4::bytes(type == fp4::NV, form, rows, (uint32_t)cols) : 0u;
 }
 
 extern "C" bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uint8_t *d_scales, uint64_t rows, uint64_t cols, uint64_t n_mat,
                                 void *d_w, uint64_t stride) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, cols) || !d_codes || !d_w || !n_mat || n_mat > 65535u || !aligned(d_w, 16) || stride % 16u ||
-        (n_mat > 1u && stride < bytes(type == NV, rows, (uint32_t)cols)) || (type == NV && !d_scales))
+        (n_mat > 1u && stride < bytes(type == NV, WEIGHTS, rows, (uint32_t)cols)) || (type == NV && !d_scales))
         return false;
     OnDevice dev;
     const uint32_t words = n_words(type == NV, (uint32_t)cols);
@@ -504,13 +539,13 @@ extern "C" bool q4_cuda_fp4_put(uint32_t type, const uint8_t *d_codes, const uin
 extern "C" bool q4_cuda_fp4_quantize(uint32_t type, uint32_t form, const float *d_x, uint64_t ld_x, float mul, uint64_t rows, uint64_t cols, void *d_q) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, cols) || form > WEIGHTS || !d_x || !d_q || ld_x < cols || !aligned(d_x, 4) || !aligned(d_q, 16)) return false;
-    return quantize<false>(type, d_x, ld_x, mul, rows, cols, d_q);
+    return quantize<false>(type, form, d_x, ld_x, mul, rows, cols, d_q);
 }
 
 extern "C" bool q4_cuda_fp4_swiglu_quantize(uint32_t type, const float *d_gu, uint64_t ld_gu, float mul, uint64_t rows, uint64_t n_ff, void *d_hq) {
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, rows, n_ff) || !d_gu || !d_hq || ld_gu < 2u * n_ff || !aligned(d_gu, 4) || !aligned(d_hq, 16)) return false;
-    return quantize<true>(type, d_gu, ld_gu, mul, rows, n_ff, d_hq);
+    return quantize<true>(type, ROWS, d_gu, ld_gu, mul, rows, n_ff, d_hq);
 }
 
 extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q, uint64_t rows, uint64_t cols, float *d_out, uint64_t ld_out) {
@@ -521,10 +556,16 @@ extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q
     const uint32_t c = (uint32_t)cols, words = n_words(type == NV, c), groups = (uint32_t)((rows + 7u) / 8u), pieces = (c + 255u) / 256u;
     const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
     const dim3 grid(groups, pieces < want ? pieces : want);
-    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, c, words, d_out, ld_out); };
+    auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, row_pitch(rows), c, words, d_out, ld_out); };
     const bool vec = aligned(d_out, 16) && ld_out % 4u == 0;
-    if (type == NV) vec ? go(values_k<true, true>) : go(values_k<true, false>);
-    else vec ? go(values_k<false, true>) : go(values_k<false, false>);
+    auto pick = [&](auto nv, auto wf) {
+        constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
+        vec ? go(values_k<N, W, true>) : go(values_k<N, W, false>);
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    if (form == ROWS) type == NV ? pick(yes(), no()) : pick(no(), no());
+    else type == NV ? pick(yes(), yes()) : pick(no(), yes());
     g_q4b_launches++;
     return q4b_launch_ok("fp4 values");
 }
@@ -544,6 +585,7 @@ extern "C" bool q4_cuda_fp4_mul(uint32_t type, const void *d_w, uint64_t w_rows,
     a.x = (const uint8_t *)d_xq;
     a.xs = a.x + code_bytes(rows, a.cols);
     a.x_rows = a.total = rows;
+    a.x_pitch = row_pitch(rows);
     a.n_expert = 1;
     a.scale = scale;
     a.dst = d_y;
@@ -558,7 +600,7 @@ extern "C" bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_ro
     using namespace fp4;
     if (!g_q4b.ok || !shape(type, w_rows, w_cols) || !shape(type, xq_rows, w_cols) || !d_w || !d_xq || !d_bounds || !d_dst || ld_dst < w_rows ||
         !n_expert || n_expert > 1024u || expert_stride_bytes % 16u ||
-        (n_expert > 1u && expert_stride_bytes < bytes(type == NV, w_rows, (uint32_t)w_cols)) || total_rows > 0x7fffffffull ||
+        (n_expert > 1u && expert_stride_bytes < bytes(type == NV, WEIGHTS, w_rows, (uint32_t)w_cols)) || total_rows > 0x7fffffffull ||
         (!d_rows && total_rows > xq_rows) || !aligned(d_w, 16) || !aligned(d_xq, 16) || !aligned(d_dst, 4))
         return false;
     if (!total_rows) return true;
@@ -572,6 +614,7 @@ extern "C" bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_ro
     a.x = (const uint8_t *)d_xq;
     a.xs = a.x + code_bytes(xq_rows, a.cols);
     a.x_rows = xq_rows;
+    a.x_pitch = row_pitch(xq_rows);
     a.rows = d_rows;
     a.bounds = d_bounds;
     a.n_expert = n_expert;

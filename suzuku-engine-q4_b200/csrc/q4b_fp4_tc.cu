@@ -3,12 +3,13 @@
 // tcgen05.mma.kind::mxf4 / mxf4nvf4 multiplies the codes and their scales as they are stored: 128 rows of x times BN rows of W,
 // 64 values of k an instruction, fp32 sums in tensor memory.  The kernel is persistent; a CTA takes tiles of
 // 128 x BN of the result (an expert's rows begin at any row; its last tile has fewer), and its warps have a task each:
-//   warp 0     copies: codes of x and W (TMA, 128-byte swizzle: 256 values of a row a stage), W's scales (bulk).  Gathered rows
-//              of x come by four (tile::gather4)
-//   warps 2-3  of experts' rows, which begin anywhere: the scales of x, word by word (cp.async)
-//   warp 1     brings a stage's scales to tensor memory (tcgen05.cp) and issues its MMAs
-//   warps 4-7  read a finished accumulator, apply the factor, transpose 32 x 32 in shared memory and store whole lines, while
-//              the MMAs fill the other one
+//   warp 0      copies of W: codes (TMA, 128-byte swizzle: 256 values of a row a stage), scales (bulk)
+//   warps 2, 3  x: codes by TMA, or where rows are gathered by cp.async (tile::gather4 took 50 cycles for four of them: 466 us where
+//               this takes 205); scales word by word (cp.async)
+//   warp 1      sees that a stage is there
+//   warp 12     brings a stage's scales to tensor memory (tcgen05.cp) and issues its MMAs
+//   warps 4-11  read a finished accumulator, apply the factor and store, while the MMAs fill the other one: 32 x 32 at a time
+//               through shared memory (TMA), of fewer rows from the registers
 // Scales in tensor memory: 128 rows' words are 4 columns (row r in lane r % 32 of column r / 32, copied to the four lane
 // quarters), a word serves 128 values of k in MXFP4 (two MMAs, told apart in the instruction descriptor), 64 in NVFP4.
 namespace fp4 {
@@ -54,7 +55,7 @@ template <bool NVF, uint32_t BN, bool PAIR> struct Cfg {
     static_assert(SF_AT + 2u * SF_COLS <= 512u && NS >= 4u && STAGE % 1024u == 0u, "layout");
 };
 struct TcMaps {
-    CUtensorMap x, w, y;                   // 32 rows of x; BH rows of an expert's W; 32 x 32 of the result
+    CUtensorMap x, x32, w, y;              // 128 and 32 rows of x; BH rows of an expert's W; 32 x 32 of the result
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, unsigned long long *bar) {
@@ -119,7 +120,7 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
     q4b_pdl_wait();
     if (tid == 0) {
-        for (uint32_t i = 0; i < C::NS; i++) mbar_init(&s.full[i], a.bounds ? 1 + 64 : 1), mbar_init(&s.ready[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
+        for (uint32_t i = 0; i < C::NS; i++) mbar_init(&s.full[i], (a.rows ? 1 : 2) + 64), mbar_init(&s.ready[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
         for (uint32_t i = 0; i < 2u; i++) mbar_init(&s.acc_full[i], 1), mbar_init(&s.acc_empty[i], PAIR ? 16 : 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -221,31 +222,22 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
     };
 
     if (warp == 0) {
-        // ---- copies ----
-        uint32_t it = 0;
-        for (uint32_t t = unit; t < all; t += units) {
-            const Tile tl = tile_of(t);
-            const uint32_t n_box = a.rows ? 0u : ((uint32_t)tl.rows + 31u) / 32u;
-            const uint32_t a0 = tl.n0 >> 7, blocks = (a.w_rows + 127u) >> 7, atoms = min(C::ATOMS, blocks - a0);
-            const bool xs_too = !a.bounds && tl.rows > 0;            // a dense product's tiles begin where a block of scales does
-            const uint32_t bytes = n_box * 4096u + C::B + (atoms + (xs_too ? 1u : 0u)) * C::WPS * 512u;
-            const uint8_t *const xs = a.xs + (uint64_t)((uint32_t)tl.m0 >> 7) * a.words * 512u;
-            const uint8_t *const ws = a.w + tl.e * a.stride + a.w_off + (uint64_t)a0 * a.words * 512u;
-            for (uint32_t k = 0; k < n_ks; k++, it++) {
-                const uint32_t sl = it % C::NS;
-                uint8_t *st = ring + sl * C::STAGE;
-                if (it >= C::NS) wait(&s.empty[sl], (it / C::NS - 1u) & 1u);
-                __syncwarp();
-                if (elect_one()) {
-                    mbar_expect_tx(&s.full[sl], bytes);
+        // ---- copies of W ----
+        if (elect_one()) {
+            uint32_t it = 0;
+            for (uint32_t t = unit; t < all; t += units) {
+                const Tile tl = tile_of(t);
+                const uint32_t a0 = tl.n0 >> 7, atoms = min(C::ATOMS, ((a.w_rows + 127u) >> 7) - a0);
+                const uint8_t *ws = a.w + tl.e * a.stride + a.w_off + (uint64_t)a0 * a.words * 512u;
+                for (uint32_t k = 0; k < n_ks; k++, it++, ws += C::WPS * 512u) {
+                    const uint32_t sl = it % C::NS;
+                    uint8_t *st = ring + sl * C::STAGE;
+                    if (it >= C::NS) wait(&s.empty[sl], (it / C::NS - 1u) & 1u);
+                    mbar_expect_tx(&s.full[sl], C::B + atoms * C::WPS * 512u);
                     tma_load_3d(st + C::A, &maps.w, &s.full[sl], (int)(k * 128u), (int)(tl.n0 + rank * C::BH), (int)tl.e);
                     for (uint32_t i = 0; i < atoms; i++)
-                        bulk_load(smem_u32(st + C::A + C::B + C::SA + i * C::WPS * 512u), ws + ((uint64_t)i * a.words + k * C::WPS) * 512u, C::WPS * 512u,
-                                  &s.full[sl]);
-                    if (xs_too) bulk_load(smem_u32(st + C::A + C::B), xs + (uint64_t)(k * C::WPS) * 512u, C::WPS * 512u, &s.full[sl]);
-                    for (uint32_t i = 0; i < n_box; i++) tma_load_2d(st + i * 4096u, &maps.x, &s.full[sl], (int)(k * 128u), tl.m0 + (int)(i * 32u));
+                        bulk_load(smem_u32(st + C::A + C::B + C::SA + i * C::WPS * 512u), ws + (uint64_t)i * a.words * 512u, C::WPS * 512u, &s.full[sl]);
                 }
-                __syncwarp();
             }
         }
     } else if (warp == 1) {
@@ -265,56 +257,70 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                 }
         }
     } else if (warp < 4u) {
-        // ---- experts' rows, which begin anywhere: the scales of x, and its codes where rows are gathered: 64 rows each.  A lane arrives when its copies have landed; who
-        // has waited for all makes them visible to the tensor cores ----
-        const uint32_t half = (warp & 1u) * 64u;
-        uint32_t it = 0;
-        for (uint32_t t = a.bounds ? unit : all; t < all; t += units) {
-            const Tile tl = tile_of(t);
-            // lane l: scales of rows l and l + 32, sixteen bytes l % 8 of the codes of rows 4 i + l / 8
-            const uint8_t *src[2];
-            uint32_t size[2], code_row[16];
-            for (uint32_t j = 0; j < 2u; j++) {
-                const int32_t r = (int32_t)(half + lane + 32u * j);
-                uint32_t x = 0;
-                bool ok = r < tl.rows;
-                if (ok) {
-                    x = (uint32_t)(a.rows ? a.rows[tl.m0 + r] : tl.m0 + r);
-                    ok = x < (uint32_t)a.x_rows;
-                }
-                src[j] = a.xs + word_at(ok ? x : 0u, 0u, a.words);
-                size[j] = ok ? 4u : 0u;
-                if (a.rows) {
+        // ---- x: scales of 64 rows a warp, word by word to their places; codes.  A lane arrives when its copies have landed ----
+        auto copies = [&](auto gathered) {
+            constexpr bool G = decltype(gathered)::value;
+            const uint32_t half = (warp & 1u) * 64u;
+            uint32_t it = 0;
+            for (uint32_t t = unit; t < all; t += units) {
+                const Tile tl = tile_of(t);
+                const int32_t mine = tl.rows - (int32_t)half;          // rows of this warp; what is behind them may hold anything
+                // lane l: scales of rows l and l + 32, sixteen bytes l % 8 of the codes of rows 4 i + l / 8
+                const uint8_t *src[2];
+                uint32_t size[2], code_row[16];
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) code_row[j * 8u + i] = __shfl_sync(0xffffffffu, ok ? x : 0xffffffffu, i * 4u + (lane >> 3));
-                }
-            }
-            for (uint32_t k = 0; k < n_ks; k++, it++) {
-                const uint32_t sl = it % C::NS;
-                if (it >= C::NS) wait(&s.empty[sl], (it / C::NS - 1u) & 1u);
-                const uint32_t st = smem_u32(ring) + sl * C::STAGE, dst = st + C::A + C::B + lane * 16u + (half >> 3);
-#pragma unroll
-                for (uint32_t w = 0; w < C::WPS; w++)
-#pragma unroll
-                    for (uint32_t j = 0; j < 2u; j++)
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + w * 512u + j * 4u),
-                                     "l"(src[j] + (uint64_t)(k * C::WPS + w) * 512u), "r"(size[j])
-                                     : "memory");
-                if (a.rows) {
-                    const uint32_t c = k * 128u + (lane & 7u) * 16u;
-                    const bool in = c < (a.cols >> 1);
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; i++) {
-                        const uint32_t r = half + i * 4u + (lane >> 3);
-                        const bool ok = in && code_row[i] != 0xffffffffu;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4)),
-                                     "l"(a.x + (ok ? (uint64_t)code_row[i] * (a.cols >> 1) + c : 0u)), "r"(ok ? 16u : 0u)
-                                     : "memory");
+                for (uint32_t j = 0; j < 2u; j++) {
+                    const int32_t r = (int32_t)(lane + 32u * j);
+                    uint32_t x = 0;
+                    bool ok = r < mine;
+                    if (ok) {
+                        x = (uint32_t)(tl.m0 + (int32_t)half + r);
+                        if (G) x = (uint32_t)a.rows[x];
+                        ok = x < (uint32_t)a.x_rows;
                     }
+                    src[j] = a.xs + (ok ? (uint64_t)x : 0u) * 4u;
+                    size[j] = ok ? 4u : 0u;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++)
+                        if (G) code_row[j * 8u + i] = __shfl_sync(0xffffffffu, ok ? x : 0xffffffffu, i * 4u + (lane >> 3));
                 }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full[sl])) : "memory");
+                for (uint32_t k = 0; k < n_ks; k++, it++) {
+                    const uint32_t sl = it % C::NS, st = smem_u32(ring) + sl * C::STAGE, dst = st + C::A + C::B + lane * 16u + (half >> 3);
+                    if (it >= C::NS) wait(&s.empty[sl], (it / C::NS - 1u) & 1u);
+#pragma unroll
+                    for (uint32_t w = 0; w < C::WPS; w++)
+#pragma unroll
+                        for (uint32_t j = 0; j < 2u; j++)
+                            if ((int32_t)(32u * j) < mine)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + w * 512u + j * 4u),
+                                             "l"(src[j] + (uint64_t)(k * C::WPS + w) * a.x_pitch * 4u), "r"(size[j])
+                                             : "memory");
+                    if (G) {
+                        const uint32_t c = k * 128u + (lane & 7u) * 16u;
+                        const bool in = c < (a.cols >> 1);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; i++) {
+                            const uint32_t r = half + i * 4u + (lane >> 3);
+                            const bool ok = in && code_row[i] != 0xffffffffu;
+                            if ((int32_t)(4u * i) < mine)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4)),
+                                             "l"(a.x + (ok ? (uint64_t)code_row[i] * (a.cols >> 1) + c : 0u)), "r"(ok ? 16u : 0u)
+                                             : "memory");
+                        }
+                    } else if (warp == 3u && elect_one()) {
+                        uint8_t *const to = ring + sl * C::STAGE;
+                        const uint32_t boxes = tl.rows > 96 ? 4u : ((uint32_t)tl.rows + 31u) / 32u;
+                        mbar_expect_tx(&s.full[sl], boxes * 4096u);
+                        if (boxes == 4u) tma_load_2d(to, &maps.x, &s.full[sl], (int)(k * 128u), tl.m0);
+                        else
+                            for (uint32_t i = 0; i < boxes; i++) tma_load_2d(to + i * 4096u, &maps.x32, &s.full[sl], (int)(k * 128u), tl.m0 + (int)(i * 32u));
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full[sl])) : "memory");
+                }
             }
-        }
+        };
+        if (a.rows) copies(std::true_type());
+        else copies(std::false_type());
     } else if (warp == 12u) {
         // ---- scales to tensor memory, MMAs ----
         if (rank == 0 && elect_one()) {
@@ -453,9 +459,9 @@ template <bool NVF, uint32_t BN, bool PAIR> bool tc_launch(const MArgs &a, uint6
     };
     const cuuint64_t xd[2] = {a.cols / 2u, a.x_rows}, xs[1] = {a.cols / 2u};
     const cuuint64_t wd[3] = {a.cols / 2u, a.w_rows, a.n_expert}, ws[2] = {a.cols / 2u, a.stride ? a.stride : code_bytes(a.w_rows, a.cols)};
-    const cuuint32_t xb[2] = {128, 32}, wb[3] = {128, C::BH, 1};
+    const cuuint32_t xb[2] = {128, 128}, x32b[2] = {128, 32}, wb[3] = {128, C::BH, 1};
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    if (!encode(&maps.x, u8, 2, a.x, xd, xs, xb) || !encode(&maps.w, u8, 3, a.w, wd, ws, wb)) return false;
+    if (!encode(&maps.x, u8, 2, a.x, xd, xs, xb) || !encode(&maps.x32, u8, 2, a.x, xd, xs, x32b) || !encode(&maps.w, u8, 3, a.w, wd, ws, wb)) return false;
     const bool vec = aligned(a.dst, 32) && a.ld % 8u == 0 && a.ld * 4u < (1ull << 40);      // whole sectors of the result
     maps.y = maps.x;
     const cuuint64_t yd[2] = {a.w_rows, a.total}, ys[1] = {a.ld * 4u};
@@ -494,21 +500,21 @@ bool tc_warm() {
 template <uint32_t BN, bool PAIR> bool tc_go(bool nv, const MArgs &a, uint64_t m_tiles) {
     return nv ? tc_launch<true, BN, PAIR>(a, m_tiles) : tc_launch<false, BN, PAIR>(a, m_tiles);
 }
-// The tile of 64, 128 or 192 rows of W with which the busiest SM has least to do (its rows and an allowance for a tile's beginning
-// and end).  Pairs of CTAs, which halve what W's rows cost in reads of the L2, for dense products of several rounds
-// of tiles: 8192 x 4096 x 2048 47.3 us, by single CTAs 50.3; for experts with fewer than 256 rows half a pair idles (8192 tokens,
-// top-10 of 512 experts, skewed: 249 us, by single CTAs 209).
+// The tile of 64, 128 or 192 rows of W with which the busiest SM has least to do: its rows and 96 for a tile's beginning and end
+// (of 64 / 128 / 192, us: 777 rows x 4099 x 2560 17 / 13.6 / 15.5; 64 tokens, top-10 of 512 experts, 1024 x 2048 127 / 75 / 73;
+// one token of them 8.7 / 6.8 / 8.0; 8192 tokens 380 / 243 / 209).  Pairs of CTAs, which halve the reads of W, for dense products of
+// four rounds of tiles and more: 8192 x 4096 x 2048 47.1 us, by single CTAs 52.0.  Of experts with fewer than 256 rows half a pair
+// idles (the 8192 tokens above: 259 us).
 bool tc_product(bool nv, const MArgs &a) {
     if (!g_tc_ready) return false;
     const uint64_t m_tiles = a.bounds ? (a.total < a.n_expert ? a.total : a.n_expert) + a.total / 128u : (a.total + 127u) / 128u;
     if (m_tiles * ((a.w_rows + 63u) / 64u) > 0x7fffffffull) return false;
-    if (getenv("Q4B_FP4_TILE")) { uint32_t v = atoi(getenv("Q4B_FP4_TILE")); if (v >= 1000) return tc_go<192, true>(nv, a, (a.bounds ? (a.total < a.n_expert ? a.total : a.n_expert) : 1) + a.total / 256u); return v == 192u ? tc_go<192, false>(nv, a, m_tiles) : v == 128u ? tc_go<128, false>(nv, a, m_tiles) : tc_go<64, false>(nv, a, m_tiles); }
     const uint64_t pairs = (a.total + 255u) / 256u;
     if (!a.bounds && pairs * ((a.w_rows + 191u) / 192u) >= 4u * (uint64_t)g_q4b.n_sm) return tc_go<192, true>(nv, a, pairs);
     uint64_t best = ~0ull;
     uint32_t bn = 192;
     for (uint32_t c = 192u; c >= 64u; c -= 64u) {
-        const uint64_t tiles = m_tiles * ((a.w_rows + c - 1u) / c), cost = (tiles + g_q4b.n_sm - 1u) / g_q4b.n_sm * (c + 64u);
+        const uint64_t tiles = m_tiles * ((a.w_rows + c - 1u) / c), cost = (tiles + g_q4b.n_sm - 1u) / g_q4b.n_sm * (c + 96u);
         if (cost < best) best = cost, bn = c;
     }
     return bn == 192u ? tc_go<192, false>(nv, a, m_tiles) : bn == 128u ? tc_go<128, false>(nv, a, m_tiles) : tc_go<64, false>(nv, a, m_tiles);

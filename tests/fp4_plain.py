@@ -35,8 +35,9 @@ def e2m1(v):
     return (code | np.where(np.signbit(v), 8, 0)).astype(np.uint8)
 
 
-def quantise(ty, v):
-    """v (float64, what a row holds after its factor) -> codes [.., n], scale bytes [.., n / block]."""
+def quantise(ty, v, exact=False):
+    """v (float64, what a row holds after its factor) -> codes [.., n], scale bytes [.., n / block].  A sixth of the largest is its
+    fp32 product with fp32's 1/6, or, of values that are no fp32 numbers (exact), the quotient."""
     n = v.shape[-1]
     x = v.reshape(*v.shape[:-1], n // BLOCK[ty], BLOCK[ty])
     with np.errstate(invalid="ignore", over="ignore"):
@@ -49,7 +50,8 @@ def quantise(ty, v):
             unit = 2.0 ** (sb - 127.0)
             nan = 255
         else:
-            want = np.minimum(top / 6.0, 448.0)
+            sixth = top / 6.0 if exact else (top.astype(np.float32) * np.float32(1.0 / 6.0)).astype(np.float64)
+            want = np.minimum(sixth, 448.0)
             up = np.clip(np.searchsorted(E4M3, want), 1, 126)
             lo, hi = want - E4M3[up - 1], E4M3[up] - want
             sb = np.where((lo < hi) | ((lo == hi) & (up % 2 == 1)), up - 1, up)

@@ -14,7 +14,7 @@ def test_quantised_values_are_nearest_of_all():
     rng = np.random.default_rng(3)
     for ty in (F.MXFP4, F.NVFP4):
         x = rng.standard_normal((50, 64)) * 3
-        codes, sb = F.quantise(ty, x)
+        codes, sb = F.quantise(ty, x, exact=True)
         v = F.values(ty, codes, sb).reshape(-1)
         unit = np.repeat(F.scale_values(ty, sb), F.BLOCK[ty], axis=-1).reshape(-1)
         every = np.concatenate([-F.MAG[::-1], F.MAG])[None, :] * unit[:, None]
@@ -40,11 +40,11 @@ def test_blocks_that_hold_no_numbers():
 def test_sizes(pkg):
     lib = pkg.capi.load()
     for ty, words in ((F.MXFP4, 2), (F.NVFP4, 4)):
-        # codes on a 256-byte boundary, then 512 bytes a word of scales of 128 rows, for columns rounded up to 256
-        for form in (F.ROWS, F.WEIGHTS):
-            assert lib.q4_cuda_fp4_bytes(ty, form, 1, 32) == 256 + words * 512
-            assert lib.q4_cuda_fp4_bytes(ty, form, 129, 2048) == 129 * 1024 + 2 * 8 * words * 512
-            assert lib.q4_cuda_fp4_bytes(ty, form, 129, 288) == -(-129 * 144 // 256) * 256 + 2 * 2 * words * 512
+        # codes on a 256-byte boundary, then words of scales for columns rounded up to 256; of four rows, or 128, at a time
+        assert lib.q4_cuda_fp4_bytes(ty, F.ROWS, 1, 32) == 256 + 256
+        assert lib.q4_cuda_fp4_bytes(ty, F.ROWS, 129, 2048) == 129 * 1024 + -(-132 * 8 * words * 4 // 256) * 256
+        assert lib.q4_cuda_fp4_bytes(ty, F.WEIGHTS, 1, 32) == 256 + words * 512
+        assert lib.q4_cuda_fp4_bytes(ty, F.WEIGHTS, 129, 288) == -(-129 * 144 // 256) * 256 + 2 * 2 * words * 512
         for form, rows, cols in ((2, 4, 64), (0, 0, 64), (0, 4, 0), (0, 4, 48), (1, 4, 65568), (1, 1 << 31, 64)):
             assert lib.q4_cuda_fp4_bytes(ty, form, rows, cols) == 0
     assert lib.q4_cuda_fp4_bytes(21, 0, 4, 64) == 0

@@ -54,7 +54,7 @@ def test_layer(dev, ty, n_tok, n_exp, topk, embd, ff):
         xq = F.values(ty, *F.quantise(ty, (dev.download(d_x, (n_tok, embd), np.float32) * np.float32(mul)).astype(np.float64)))
         atok = dev.download(d_atok, (rows,), np.int32)
         gu, pd = dev.download(d_gu, (rows, 2 * ff), np.float32), dev.download(d_pd, (rows, embd), np.float32)
-        hq = F.values(ty, *F.quantise(ty, F.swiglu(gu, mul)))       # of the gate and up values that the device has
+        hq = F.values(ty, *F.quantise(ty, F.swiglu(gu, mul), exact=True))       # of the gate and up values that the device has
         scale = 1.0 / mul ** 2
         for e in range(n_mat):
             lo, hi = bounds[e], bounds[e + 1]
@@ -66,7 +66,7 @@ def test_layer(dev, ty, n_tok, n_exp, topk, embd, ff):
         want = np.zeros((n_tok, embd))
         for t in range(n_tok):
             for e, w in list(zip(ids[t], wts[t])) + [(n_exp, 1.0)]:
-                h = F.values(ty, *F.quantise(ty, F.swiglu((xq[t] @ w_gu[e].T * scale)[None].astype(np.float32), mul)))[0]
+                h = F.values(ty, *F.quantise(ty, F.swiglu((xq[t] @ w_gu[e].T * scale)[None].astype(np.float32), mul), exact=True))[0]
                 want[t] += float(w) * (h @ w_dn[e].T * scale)
         assert np.linalg.norm(y - want) <= 1e-2 * np.linalg.norm(want)
         return y
