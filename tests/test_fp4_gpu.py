@@ -178,7 +178,9 @@ def _check(got, x, w, scale, ty):
 @pytest.mark.parametrize("rows,w_rows,cols,extra", [
     (1, 1, 32, 0), (1, 128, 256, 0), (2, 31, 96, 3), (1, 4099, 2048, 0), (3, 129, 544, 0), (5, 200, 1024, 8), (8, 512, 2048, 0), (9, 130, 288, 1),
     (16, 1000, 64, 0), (17, 192, 256, 0), (33, 193, 320, 7), (64, 384, 2048, 0), (100, 65, 512, 0), (128, 448, 736, 0), (129, 1024, 1024, 0),
-    (300, 513, 2560, 0), (777, 640, 352, 16), (1500, 257, 4096, 0)])
+    (300, 513, 2560, 0), (777, 640, 352, 16), (1500, 257, 4096, 0),
+    # enough tiles for pairs of CTAs: a last pair with and without rows for its second one, whole and ragged columns
+    (4111, 6801, 96, 0), (4352, 7104, 320, 8), (4190, 7000, 32, 4)])
 def test_mul(dev, ty, rows, w_rows, cols, extra):
     rng = np.random.default_rng(rows * 7 + cols)
     w, d_w, _ = _weights(dev, rng, ty, 1, w_rows, cols)
