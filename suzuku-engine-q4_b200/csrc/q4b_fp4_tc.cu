@@ -25,7 +25,6 @@ using mmqtc::smem_u32;
 using mmqtc::tc_fence_after;
 using mmqtc::tc_fence_before;
 using mmqtc::tma_load_2d;
-using mmqtc::tmem_ld_wait;
 
 constexpr uint32_t ERR_FP4 = 1u << 20;
 constexpr uint32_t KSTAGE = 256u;
@@ -92,12 +91,14 @@ __device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint
     }
 #undef Q4B_FP4_MMA
 }
+// 32 columns of a lane's row, and the wait for them (in one statement, so that nothing is computed from them before)
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *f) {
     uint32_t *v = reinterpret_cast<uint32_t *>(f);
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
           "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
           "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
@@ -118,12 +119,20 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
     TcSmem &s = *reinterpret_cast<TcSmem *>(smem_raw + C::NS * C::STAGE + OUT);
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t rank = PAIR ? blockIdx.x & 1u : 0u, unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
-    q4b_pdl_wait();
     if (tid == 0) {
         for (uint32_t i = 0; i < C::NS; i++) mbar_init(&s.full[i], (a.rows ? 1 : 2) + 64), mbar_init(&s.ready[i], PAIR ? 2 : 1), mbar_init(&s.empty[i], 1);
         for (uint32_t i = 0; i < 2u; i++) mbar_init(&s.acc_full[i], 1), mbar_init(&s.acc_empty[i], PAIR ? 16 : 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (!a.bounds && warp == 1u && elect_one()) {       // a dense product's first stages of W, into the L2, before the kernel ahead is waited for
+        const uint32_t n = (a.w_rows + BN - 1u) / BN, stages = min((a.cols + KSTAGE - 1u) / KSTAGE, C::NS);
+        for (uint32_t k = 0; k < stages; k++)
+            asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(&maps.w), "r"((int)(k * 128u)),
+                         "r"((int)(unit % n * BN + rank * C::BH)), "r"(0)
+                         : "memory");
+    }
+    __syncwarp();
+    q4b_pdl_wait();
     if (warp == 0) {
         if (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)) : "memory");
@@ -385,7 +394,6 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                 const uint32_t col = tl.n0 + c0;
                 float v[32];
                 tmem_ld32(tmem + ((32u * q) << 16) + acc * BN + c0, v);
-                tmem_ld_wait();
 #pragma unroll
                 for (uint32_t i = 0; i < 32u; i++) v[i] = there ? v[i] * f : 0.f;
                 if (mine < 32 && vec && col + 32u <= a.w_rows) {       // fewer rows: each from its lane, in whole sectors
