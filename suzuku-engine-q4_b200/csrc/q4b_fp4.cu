@@ -497,8 +497,8 @@ template <bool SWIGLU> bool quantize(uint32_t type, uint32_t form, const float *
 bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
 
 // Few rows on the CUDA cores while their work is that of two CTAs of 2048 columns an SM, else on the tensor cores.  us with the
-// quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 7.0, 2 rows 6.5 / 7.0, 3 rows 9.1 / 7.0;
-// 8192 x 2560 1 row 8.5 / 8.0; 1024 x 1024 1 row 3.9 / 5.3, 8 rows 4.4 / 5.4.
+// quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 6.6, 2 rows 6.5 / 6.6, 3 rows 9.1 / 6.6;
+// 8192 x 2560 1 row 8.5 / 7.6; 1024 x 1024 1 row 3.9 / 5.1, 8 rows 4.4 / 5.2.
 bool product(uint32_t type, MArgs &a) {
     OnDevice dev;
     const uint64_t ctas = a.total * ((a.w_rows + 127u) / 128u * 4u);

@@ -131,6 +131,11 @@ template <bool NVF, uint32_t BN, bool PAIR> __global__ void __launch_bounds__(TH
                          "r"((int)(unit % n * BN + rank * C::BH)), "r"(0)
                          : "memory");
     }
+    // Rows that a tile does not have are multiplied all the same: by zeros while no tile had them, which takes less power than by what
+    // shared memory holds, and a card at its power limit lowers its clock (64 tokens, top-10 of 512 experts: 78.5 us instead of 82).
+    for (uint32_t i = 0; i < C::NS; i++)
+        for (uint32_t k = tid; k < C::A / 16u; k += THREADS) *reinterpret_cast<uint4 *>(ring + i * C::STAGE + k * 16u) = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     q4b_pdl_wait();
     if (warp == 0) {
