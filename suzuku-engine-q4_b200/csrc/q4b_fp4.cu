@@ -258,32 +258,45 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
     }
 }
 
-// A quantised matrix as the values that it stands for: a warp 256 values of a row at a time.
-template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t pitch, uint32_t cols, uint32_t words,
-                                                                                      float *out, uint64_t ld) {
+// A quantised matrix as the values that it stands for: a warp 256 values of a row at a time, eight a lane, which are a sector (VEC) of the
+// result.  Bound by its writes.
+template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) values_k(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t pitch,
+                                                                                      uint32_t cols, uint32_t words, float *out, uint64_t ld) {
+    constexpr int U = 4;
     q4b_pdl_wait();
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t row = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
     if (row >= rows) return;
-#pragma unroll 2
-    for (uint32_t c0 = blockIdx.y * 256u; c0 < cols; c0 += gridDim.y * 256u) {
+    const uint32_t step = gridDim.y * 256u;
+    for (uint32_t c0 = blockIdx.y * 256u + lane * 8u; c0 < cols; c0 += U * step) {
+        uint32_t q[U], sb[U];
 #pragma unroll
-        for (uint32_t h = 0; h < 2u; h++) {          // four values a lane, so that a store is whole lines
-            const uint32_t c = c0 + h * 128u + lane * 4u;
-            if (c >= cols) continue;
-            const uint32_t b = c >> (NVF ? 4 : 5);
-            const float s = scale_value<NVF>(scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)]) * 0.5f;
-            const uint32_t q = *reinterpret_cast<const uint16_t *>(codes + row * (cols >> 1) + (c >> 1));
-            const uint32_t m = prmt(MAG_LO, MAG_HI, q & 0x7777u);
-            float v[4];
+        for (int k = 0; k < U; k++) {
+            const uint32_t c = c0 + k * step, b = c >> (NVF ? 4 : 5);
+            if (c >= cols) break;
+            q[k] = *reinterpret_cast<const uint32_t *>(codes + row * (cols >> 1) + (c >> 1));
+            sb[k] = scales[word_at<WF>(row, b >> 2, words, pitch) + (b & 3u)];
+        }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float f = (float)((m >> (8 * k)) & 0xffu) * s;
-                v[k] = (q >> (4 * k)) & 8u ? -f : f;
+        for (int k = 0; k < U; k++) {
+            const uint32_t c = c0 + k * step;
+            if (c >= cols) break;
+            const float s = scale_value<NVF>(sb[k]) * 0.5f;
+            const uint32_t m[2] = {prmt(MAG_LO, MAG_HI, q[k] & 0x7777u), prmt(MAG_LO, MAG_HI, (q[k] >> 16) & 0x7777u)};
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float f = (float)((m[i >> 2] >> (8 * (i & 3))) & 0xffu) * s;
+                v[i] = (q[k] >> (4 * i)) & 8u ? -f : f;
             }
             float *o = out + row * ld + c;
-            if (VEC) *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
-            else o[0] = v[0], o[1] = v[1], o[2] = v[2], o[3] = v[3];
+            if (VEC)
+                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+                             "f"(v[5]), "f"(v[6]), "f"(v[7])
+                             : "memory");
+            else
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = v[i];
         }
     }
 }
@@ -558,7 +571,7 @@ extern "C" bool q4_cuda_fp4_values(uint32_t type, uint32_t form, const void *d_q
     const uint32_t want = (8u * (uint32_t)g_q4b.n_sm + groups - 1u) / groups;
     const dim3 grid(groups, pieces < want ? pieces : want);
     auto go = [&](auto k) { q4b_launch(k, grid, dim3(256), 0, g_q4b.stream, codes, scales, rows, row_pitch(rows), c, words, d_out, ld_out); };
-    const bool vec = aligned(d_out, 16) && ld_out % 4u == 0;
+    const bool vec = aligned(d_out, 32) && ld_out % 8u == 0;
     auto pick = [&](auto nv, auto wf) {
         constexpr bool N = decltype(nv)::value, W = decltype(wf)::value;
         vec ? go(values_k<N, W, true>) : go(values_k<N, W, false>);
