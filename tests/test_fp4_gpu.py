@@ -178,7 +178,7 @@ def _check(got, x, w, scale, ty):
 @pytest.mark.parametrize("rows,w_rows,cols,extra", [
     (1, 1, 32, 0), (1, 128, 256, 0), (2, 31, 96, 3), (1, 4099, 2048, 0), (3, 129, 544, 0), (5, 200, 1024, 8), (8, 512, 2048, 0), (9, 130, 288, 1),
     (16, 1000, 64, 0), (17, 192, 256, 0), (33, 193, 320, 7), (64, 384, 2048, 0), (100, 65, 512, 0), (128, 448, 736, 0), (129, 1024, 1024, 0),
-    (300, 513, 2560, 0), (777, 640, 352, 16), (1500, 257, 4096, 0),
+    (300, 513, 2560, 0), (777, 640, 352, 16), (1500, 257, 4096, 0), (1, 33, 65536, 0), (140, 130, 65536, 0),
     # enough tiles for pairs of CTAs: a last pair with and without rows for its second one, whole and ragged columns
     (4111, 6801, 96, 0), (4352, 7104, 320, 8), (4190, 7000, 32, 4)])
 def test_mul(dev, ty, rows, w_rows, cols, extra):
@@ -363,3 +363,38 @@ def test_nothing_is_written_behind_a_buffer(dev):
                 x = np.ones((rows, cols), np.float32)
                 assert lib.q4_cuda_fp4_quantize(ty, form, dev.upload(x), cols, 1.0, rows, cols, d)
                 assert (dev.download(d, (size + 512,), np.uint8)[size:] == 0xAB).all()
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_offsets_beyond_32_bits(dev, ty):
+    """Rows whose place in the result, or in the values read back, is behind 2^31 elements; of each the last rows are looked at."""
+    lib, cols, w_rows, rows = dev.lib, 64, 32768, 70000
+    rng = np.random.default_rng(11)
+    w, d_w, _ = _weights(dev, rng, ty, 1, w_rows, cols)
+    x, d_x = _rows(dev, rng, ty, rows, cols)
+    d_y = dev.malloc(4 * rows * w_rows)
+    for gather in (False, True):
+        assert lib.q4_hip_fill(d_y, 0.0, rows * w_rows)
+        pick = np.arange(rows)[::-1] if gather else np.arange(rows)
+        d_rows, d_b = dev.upload(pick.astype(np.int32)), dev.upload(np.array([0, rows], np.int32))
+        if gather:
+            ok = lib.q4_cuda_fp4_mul_id(ty, d_w, w_rows, cols, 0, 1, d_x, rows, d_rows, d_b, rows, 1.0, None, d_y, w_rows)
+        else:
+            ok = lib.q4_cuda_fp4_mul(ty, d_w, w_rows, cols, d_x, rows, 1.0, d_y, w_rows)
+        assert ok
+        for r in (0, 65535, 65536, 69990):
+            got = dev.download(d_y + 4 * r * w_rows, (10, w_rows), np.float32)
+            _check(got, x[pick[r:r + 10]], w[0], 1.0, ty)
+        dev.free(d_rows), dev.free(d_b)
+    # the result as a matrix of fp32 rows: quantised and read back
+    n = 2048
+    big = rows * w_rows // n
+    d_q, _ = _buffer(dev, ty, F.ROWS, big, n)
+    assert lib.q4_cuda_fp4_quantize(ty, F.ROWS, d_y, n, 1.0, big, n, d_q)
+    tail = dev.download(d_y + 4 * (big - 7) * n, (7, n), np.float32)
+    assert lib.q4_cuda_fp4_values(ty, F.ROWS, d_q, big, n, d_y, n)
+    got = dev.download(d_y + 4 * (big - 7) * n, (7, n), np.float32)
+    np.testing.assert_array_equal(got, F.values(ty, *F.quantise(ty, tail.astype(np.float64))).astype(np.float32))
+    for d in (d_w, d_x, d_y, d_q):
+        dev.free(d)
+    assert lib.q4_cuda_device_error() == 0

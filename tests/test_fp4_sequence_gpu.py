@@ -61,7 +61,10 @@ def test_layer(dev, ty, n_tok, n_exp, topk, embd, ff):
             a, h = xq[atok[lo:hi]], hq[lo:hi]
             assert (np.abs(gu[lo:hi] - a @ w_gu[e].T * scale) <= F.product_bound(a, w_gu[e], scale, embd // F.BLOCK[ty])).all()
             assert (np.abs(pd[lo:hi] - h @ w_dn[e].T * scale) <= F.product_bound(h, w_dn[e], scale, ff // F.BLOCK[ty])).all()
-        # the layer as a whole, from the picks and the weights: a value of h next to a border may fall on its other side
+        # the layer as a whole, from the picks and the weights.  The device's gate and up values are fp32 sums, up to 1e-6 off, and a
+        # value of h so near to a border falls on its other side: some four in a million, of half a million values at most, and
+        # each moves one of n_ff values of a row by a third at most.  Three of them in one row of 128: 3 / 3 / sqrt(128) of its norm,
+        # an eighth of the picks' share of one token of 700; of one token alone none is expected, and one would be 1 / 3 / sqrt(32).
         y = dev.download(d_y, (n_tok, embd), np.float32)
         want = np.zeros((n_tok, embd))
         for t in range(n_tok):
