@@ -27,19 +27,27 @@ __device__ __forceinline__ void count(const Args &a, uint32_t cta, uint32_t ctas
     if (threadIdx.x == 0) *n_live = 0;
     __syncthreads();
     int32_t live = 0;
-    for (uint32_t t = cta * blockDim.x + threadIdx.x; t < a.n_tok; t += ctas * blockDim.x) {
-        const bool ok = !a.valid || a.valid[t];
-        live += ok;
-        const int32_t *ids = a.ids + (uint64_t)t * a.topk;
-        for (uint32_t k0 = 0; k0 < a.topk; k0 += 16u) {
-            int32_t e[16];
+    const uint32_t step = ctas * blockDim.x;
+    for (uint32_t t0 = cta * blockDim.x + threadIdx.x; t0 < a.n_tok; t0 += 2u * step)        // two tokens' loads at a time
+        for (uint32_t k0 = 0; k0 < a.topk; k0 += 10u) {
+            int32_t e[2][10];
+            bool ok[2];
 #pragma unroll
-            for (uint32_t k = 0; k < 16u; k++) e[k] = k0 + k < a.topk ? ids[k0 + k] : -1;
+            for (uint32_t h = 0; h < 2u; h++) {
+                const uint32_t t = t0 + h * step;
+                ok[h] = t < a.n_tok;
 #pragma unroll
-            for (uint32_t k = 0; k < 16u; k++)
-                if (ok && (uint32_t)e[k] < a.n_exp) atomicAdd(&hist[e[k]], 1);
+                for (uint32_t k = 0; k < 10u; k++) e[h][k] = ok[h] && k0 + k < a.topk ? a.ids[(uint64_t)t * a.topk + k0 + k] : -1;
+                if (ok[h] && a.valid) ok[h] = a.valid[t] != 0;
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                live += ok[h] && k0 == 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 10u; k++)
+                    if (ok[h] && (uint32_t)e[h][k] < a.n_exp) atomicAdd(&hist[e[h][k]], 1);
+            }
         }
-    }
     live = __reduce_add_sync(0xffffffffu, live);
     if ((threadIdx.x & 31u) == 0 && live) atomicAdd(n_live, live);
     __syncthreads();
@@ -196,8 +204,13 @@ template <int NV, bool VEC> __global__ void __launch_bounds__(32u * warps(NV)) r
     for (uint32_t e = threadIdx.x; e < a.n_exp; e += blockDim.x) {
         float s = alone ? sum[1][e] : 0.f;
         if (!alone)
-#pragma unroll 8
-            for (uint32_t c = 0; c < clusters; c++) s += __ldcg(a.part + (uint64_t)c * a.n_exp + e);
+            for (uint32_t c0 = 0; c0 < clusters; c0 += 16u) {
+                float p[16];
+#pragma unroll
+                for (uint32_t c = 0; c < 16u; c++) p[c] = c0 + c < clusters ? __ldcg(a.part + (uint64_t)(c0 + c) * a.n_exp + e) : 0.f;
+#pragma unroll
+                for (uint32_t c = 0; c < 16u; c++) s += p[c];
+            }
         const float p = s * inv_n;
         if (a.counts) a.counts[e] = total[e];
         if (a.prob) a.prob[e] = p;
