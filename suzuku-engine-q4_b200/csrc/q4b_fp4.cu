@@ -149,14 +149,14 @@ __device__ __forceinline__ double swiglu64(double g, double u, double mul) { ret
 template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uint32_t &sb) {
     double a = 0.0;
     bool bad = false;
-    for (int i = 0; i < 8; i++) a = fmax(a, fabs(v[i])), bad |= !(fabs((double)(float)v[i]) <= 3.402823466e38);
+    for (int i = 0; i < 8; i++) a = fmax(a, fabs(v[i])), bad |= !isfinite((float)v[i]);
     if (bad) a = __longlong_as_double(0x7ff8000000000000ll);
     unsigned long long u = (unsigned long long)__double_as_longlong(a);
     u = max(u, __shfl_xor_sync(0xffffffffu, u, 1));
     if (!NVF) u = max(u, __shfl_xor_sync(0xffffffffu, u, 2));
     a = __longlong_as_double((long long)u);
     double unit;
-    if (!(a <= 3.402823466e38)) {
+    if (a != a) {
         sb = NVF ? 0x7fu : 255u;
         return 0u;
     }
@@ -183,8 +183,7 @@ template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uin
 }
 
 // A warp takes 256 values of a row at a time, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same
-// columns of eight rows that follow one another; U such pieces of a row are
-// loaded before the first is quantised (two of 8192 x 2048 14.6 us, 5.3 TB/s; one 16.4, four 16.0; with SwiGLU 22528 x 512 two 19.4 us,
+// columns of eight rows that follow one another; U such pieces of a row are loaded before the first is quantised (two of 8192 x 2048 14.6 us, 5.3 TB/s; one 16.4, four 16.0; with SwiGLU 22528 x 512 two 19.4 us,
 // 5.1 TB/s, one 20.3).  Bound by those loads and, with SwiGLU, by issue slots.
 template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
     constexpr int U = 2;
@@ -509,6 +508,7 @@ template <bool SWIGLU> bool quantize(uint32_t type, uint32_t form, const float *
 }
 
 bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
+static bool g_tc_ready = false;
 
 // Few rows on the CUDA cores while their work is that of two CTAs of 2048 columns an SM, else on the tensor cores.  us with the
 // quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 6.6, 2 rows 6.5 / 6.6, 3 rows 9.1 / 6.6;
@@ -516,7 +516,7 @@ bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
 bool product(uint32_t type, MArgs &a) {
     OnDevice dev;
     const uint64_t ctas = a.total * ((a.w_rows + 127u) / 128u * 4u);
-    if (ctas * a.cols > 2u * (uint64_t)g_q4b.n_sm * 2048u) return tc_product(type == NV, a);
+    if (g_tc_ready && ctas * a.cols > 2u * (uint64_t)g_q4b.n_sm * 2048u) return tc_product(type == NV, a);
     const dim3 grid((a.w_rows + 127u) / 128u * 4u, (unsigned)(a.total < 65535u ? a.total : 65535u));
     if (type == NV) q4b_launch(few_k<true>, grid, dim3(256), 0, g_q4b.stream, a);
     else q4b_launch(few_k<false>, grid, dim3(256), 0, g_q4b.stream, a);

@@ -498,7 +498,6 @@ template <bool NVF, uint32_t BN, bool PAIR> bool tc_launch(const MArgs &a, uint6
     return q4b_launch_ok("fp4 product");
 }
 
-static bool g_tc_ready = false;
 template <uint32_t BN, bool PAIR> bool tc_attr() {
     return cudaFuncSetAttribute(tc_k<false, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<false, BN, PAIR>::SMEM) == cudaSuccess &&
            cudaFuncSetAttribute(tc_k<true, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<true, BN, PAIR>::SMEM) == cudaSuccess;
@@ -519,7 +518,6 @@ template <uint32_t BN, bool PAIR> bool tc_go(bool nv, const MArgs &a, uint64_t m
 // four rounds of tiles and more: 8192 x 4096 x 2048 47.1 us, by single CTAs 52.0.  Of experts with fewer than 256 rows half a pair
 // idles (the 8192 tokens above: 259 us).
 bool tc_product(bool nv, const MArgs &a) {
-    if (!g_tc_ready) return false;
     const uint64_t m_tiles = a.bounds ? (a.total < a.n_expert ? a.total : a.n_expert) + a.total / 128u : (a.total + 127u) / 128u;
     if (m_tiles * ((a.w_rows + 63u) / 64u) > 0x7fffffffull) return false;
     const uint64_t pairs = (a.total + 255u) / 256u;

@@ -24,7 +24,7 @@ void q4b_elem_shutdown();
 bool q4b_mmvq_warm();    // q4b_mmvq.cu: quantised rows of the dense 8-bit product
 bool q4b_route_small_warm();   // q4b_decode.cu: counters of the one-launch routing
 void q4b_route_small_shutdown();
-bool q4b_fp4_warm();           // q4b_fp4_tc.cu: shared-memory limits of the products
+bool q4b_fp4_warm();           // q4b_fp4_tc.cu: shared-memory limits of the tensor-core products
 bool q4b_balance_warm();       // q4b_balance.cu: sums of the balance loss
 void q4b_balance_shutdown();
 void q4b_mmvq_shutdown();
@@ -248,8 +248,9 @@ bool alloc_scratch() {
     Q4B_CHECK(cudaMalloc(&s.hbuf, nq * sizeof(float)));
     q4b_router_tc_warm();
     q4b_mmq_tc_warm();  // without it the grouped product stays on the CUDA cores
+    q4b_fp4_warm();     // ... and so do those of 4-bit floating point
     return q4b_fused_warm() && q4b_window_warm() && q4b_elem_warm() && q4b_mmvq_warm() && q4b_route_small_warm() &&
-           q4b_fp4_warm() && q4b_balance_warm();
+           q4b_balance_warm();
 }
 
 }  // namespace

@@ -147,7 +147,7 @@ def test_swiglu_quantize_is_that_of_the_exact_values(dev, ty, rows, n_ff, extra,
     g, u = gu[:, :n_ff], gu[:, n_ff:]
     mul = float(np.float32(mul))
     hard = [(-88.0, 1.0), (-95.0, 1e20), (-104.0, 1e30), (np.nan, 1.0), (np.inf, 1.0), (1.0, -np.inf), (0.0, 5.0), (3e38, 0.9), (3e38, 7.0),
-            (-120.0, 3.0), (1e-30, 1e-9), (1e-30, 1e-20), (-0.0, 2.0), (70.0, 6.0), (-np.inf, 1.0)]
+            (-120.0, 3.0), (1e-30, 1e-9), (1e-30, 1e-20), (-0.0, 2.0), (70.0, 6.0), (-np.inf, 1.0), (F.FMAX, 1.0), (F.FMAX, 0.999), (-60.0, F.FMAX)]
     for i, (a, b) in enumerate(hard):
         r, c = (i * 5) % rows, (i * 64) % n_ff
         if rows * n_ff > 32 * len(hard):
