@@ -179,6 +179,8 @@ def _check(got, x, w, scale, ty):
     (1, 1, 32, 0), (1, 128, 256, 0), (2, 31, 96, 3), (1, 4099, 2048, 0), (3, 129, 544, 0), (5, 200, 1024, 8), (8, 512, 2048, 0), (9, 130, 288, 1),
     (16, 1000, 64, 0), (17, 192, 256, 0), (33, 193, 320, 7), (64, 384, 2048, 0), (100, 65, 512, 0), (128, 448, 736, 0), (129, 1024, 1024, 0),
     (300, 513, 2560, 0), (777, 640, 352, 16), (1500, 257, 4096, 0), (1, 33, 65536, 0), (140, 130, 65536, 0),
+    # more of the tensor cores' (calls of little work are the CUDA cores'): a column tile's and a row tile's end, few columns
+    (1300, 513, 32, 0), (700, 129, 352, 1), (40, 1000, 544, 0), (9, 4099, 544, 0), (33, 2311, 320, 9), (127, 640, 96, 0), (600, 65, 512, 7),
     # enough tiles for pairs of CTAs: a last pair with and without rows for its second one, whole and ragged columns
     (4111, 6801, 96, 0), (4352, 7104, 320, 8), (4190, 7000, 32, 4)])
 def test_mul(dev, ty, rows, w_rows, cols, extra):
@@ -196,7 +198,7 @@ def test_mul(dev, ty, rows, w_rows, cols, extra):
     assert dev.lib.q4_cuda_device_error() == 0
 
 
-@pytest.mark.parametrize("rows", [1, 40, 200])
+@pytest.mark.parametrize("rows", [1, 40, 200, 400])
 def test_mul_scales_far_apart(dev, rows):
     """Powers of two whose product is an ordinary number although neither is, and NaN blocks: a row of the weights or of
     the activations, and nothing beside it."""
@@ -225,7 +227,10 @@ def test_mul_scales_far_apart(dev, rows):
 
 CASES = [  # experts, w_rows, cols, rows of each expert
     (4, 128, 256, [1, 0, 2, 1]), (3, 200, 96, [0, 0, 5]), (6, 64, 512, [0, 3, 0, 0, 9, 0]), (2, 513, 544, [33, 130]), (5, 384, 1024, [128, 1, 129, 0, 64]),
-    (9, 256, 288, [7, 300, 0, 2, 41, 1, 1, 16, 90]), (1, 192, 2048, [500]), (70, 192, 256, [i % 5 for i in range(70)]), (1024, 32, 32, [1] * 1024)]
+    (9, 256, 288, [7, 300, 0, 2, 41, 1, 1, 16, 90]), (1, 192, 2048, [500]), (70, 192, 256, [i % 5 for i in range(70)]), (1024, 32, 32, [1] * 1024),
+    # more of the tensor cores': few rows of large matrices, more tiles of rows than their table has
+    (6, 2100, 1024, [0, 3, 0, 0, 9, 0]), (70, 640, 512, [i % 5 for i in range(70)]), (1024, 200, 64, [1 + i % 3 for i in range(1024)]),
+    (3, 1500, 96, [0, 260, 131])]
 
 
 @pytest.mark.parametrize("ty", TYPES)
@@ -266,10 +271,11 @@ def test_mul_id(dev, ty, gather, case):
 
 @pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("first,last,total", [(3, 20, 30), (0, 30, 17), (5, 5, 12), (130, 270, 400)])
-def test_mul_id_leaves_rows_of_nobody_alone(dev, ty, first, last, total):
+@pytest.mark.parametrize("w_rows,cols", [(160, 128), (4000, 512)])
+def test_mul_id_leaves_rows_of_nobody_alone(dev, ty, first, last, total, w_rows, cols):
     """Bounds that begin behind row 0 or end before the last row, and rows behind total_rows."""
     rng = np.random.default_rng(first + total)
-    n, w_rows, cols = 3, 160, 128
+    n = 3
     w, d_w, stride = _weights(dev, rng, ty, n, w_rows, cols)
     rows = max(total, last)
     x, d_x = _rows(dev, rng, ty, rows, cols)
