@@ -639,7 +639,8 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  *   Q4_FP4_WEIGHTS  weights: what they take as d_w; the matrices of several experts stand a stride apart
  *   put              n_mat matrices of a checkpoint -> weights at d_w + i * stride.  d_codes [n_mat][rows][cols / 2], value 2 i
  *                    in the low half of byte i; d_scales [n_mat][rows][cols / 32 or 16].  d_scales == NULL (MXFP4): d_codes
- *                    holds ggml blocks of 17 bytes, the scale first, values j and j + 16 in the halves of byte j
+ *                    holds ggml blocks of 17 bytes, the scale first, values j and j + 16 in the halves of byte j.  A
+ *                    negative e4m3 scale (0xff: NaN) turns its block's signs round and is kept without its own
  *   quantize         fp32 rows, ld_x floats apart, -> either form
  *   swiglu_quantize  silu(gu[r][k]) * gu[r][n_ff + k] * mul -> rows form.  Scales and codes are those of the exact
  *                    values (and of max / 6; one that fp32 leaves next to a border is computed again in 64 bits)

@@ -3,7 +3,7 @@
 //
 // A value is a sign and a magnitude out of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (E2M1) times its block's scale:
 //   MXFP4  32 values share 2^(b - 127), one byte b (255 = NaN)
-//   NVFP4  16 values share an e4m3 number, one byte (0x7f = NaN)
+//   NVFP4  16 values share an e4m3 number without its sign, one byte (0x7f = NaN)
 // A quantised [rows][cols] matrix begins with the codes, row after row, value 2 i in the low half of byte i.  Behind them (on the
 // next 256-byte boundary) stand the scales as words of four bytes, the four blocks of a row that follow one another (128
 // values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there):
@@ -302,7 +302,8 @@ template <bool NVF, bool WF, bool VEC> __global__ void __launch_bounds__(256) va
 
 // Matrices in the form of a checkpoint to the weights order: a thread takes 16 bytes of codes (32 values), and the one that has a
 // word's first block its scales.  scales == NULL: ggml blocks of 17 bytes, the scale and then codes j (low half) and j + 16 (high half)
-// in byte j.
+// in byte j.  The tensor cores' e4m3 scales have no sign: a negative one gives its sign to the block's codes, so that a value is the same
+// to every reader of the buffer.
 template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *codes, const uint8_t *scales, uint32_t rows, uint32_t cols, uint32_t words,
                                                                  uint8_t *w, uint64_t stride, uint64_t scale_off, bool vec) {
     q4b_pdl_wait();
@@ -320,7 +321,7 @@ template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *
                 const uint32_t b = p / PER * 4u + j;
                 if (b < nb) sw |= (uint32_t)(scales ? scales[r * nb + b] : codes[(r * nb + b) * 17u]) << (8u * j);
             }
-            *reinterpret_cast<uint32_t *>(to + scale_off + word_at<true>(row, p / PER, words, 0)) = sw;
+            *reinterpret_cast<uint32_t *>(to + scale_off + word_at<true>(row, p / PER, words, 0)) = NVF ? sw & 0x7f7f7f7fu : sw;
         }
         if (p * 32u >= cols) continue;
         uint32_t q[4] = {0, 0, 0, 0};
@@ -336,6 +337,10 @@ template <bool NVF> __global__ void __launch_bounds__(256) put_k(const uint8_t *
                 q[k >> 2] |= ((a & 15u) | ((b & 15u) << 4)) << (8u * (k & 3u));
                 q[2u + (k >> 2)] |= ((a >> 4) | (b & 0xf0u)) << (8u * (k & 3u));
             }
+        }
+        if (NVF) {           // (p's two blocks; each is there, cols being a multiple of 32)
+            if (scales[r * nb + 2u * p] & 0x80u) q[0] ^= 0x88888888u, q[1] ^= 0x88888888u;
+            if (scales[r * nb + 2u * p + 1u] & 0x80u) q[2] ^= 0x88888888u, q[3] ^= 0x88888888u;
         }
         *reinterpret_cast<uint4 *>(to + (uint64_t)row * (cols >> 1) + p * 16u) = make_uint4(q[0], q[1], q[2], q[3]);
     }
