@@ -205,6 +205,7 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
             *reinterpret_cast<uint32_t *>(a.scales + word_at<WF>(row, (c0 >> (NVF ? 6 : 7)) + lane / (NVF ? 8u : 16u), a.words, a.pitch)) = w;
     };
     const uint32_t step = gridDim.y * 256u;
+    const float low = fabsf(a.mul) > 0x1p50f ? INFINITY : 1e-20f;
     for (uint32_t c0 = blockIdx.y * 256u; c0 < a.cols; c0 += U * step) {
         float v[U][8], u[U][8];
 #pragma unroll
@@ -227,19 +228,21 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
             }
             // fp32 is off by at most 2 steps of 2^-23 for the exponential, half a one for the sum, 2 for the quotient (its divisor is
             // below 2^126), half a one each for two products and for the unit's, 1 for its inverse: below 2^-20.  Where that leaves
-            // the scale or a code in doubt, or fp32's range is left, the warp computes in 64 bits.
+            // the scale or a code in doubt, or fp32's range is left, the warp computes in 64 bits.  A product g u or a quotient that has
+            // lost bits (below 2^-126) is below 2^-76 after a mul of up to 2^50, and then a zero in a block whose largest is 1e-20 or more
+            // (a code's lowest border is a 32nd of it at least); a block with less is in doubt, unless a factor of each of its products is 0.
             constexpr float LO = 1.f - 0x1p-20f, HI = 1.f + 0x1p-20f;
             float t[8];
             bool doubt = false;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float g = v[k][i];
-                t[i] = __fdividef(g, 1.f + expf(-g)) * u[k][i] * a.mul;
+                t[i] = __fdividef(g * u[k][i], 1.f + expf(-g)) * a.mul;
                 doubt |= g < -80.f;
             }
             const float top = block_max<NVF>(max8(t));
             uint32_t sb = scale_byte<NVF>(top * LO);
-            doubt |= scale_byte<NVF>(top * HI) != sb || top > 1e38f || (top > 0.f && top < 1e-30f);
+            doubt |= scale_byte<NVF>(top * HI) != sb || !(top <= 1e38f) || top < low;
             const float inv = inverse<NVF>(sb);
             float lo[8], hi[8];
 #pragma unroll
@@ -248,9 +251,13 @@ template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bou
             doubt |= q != encode8(hi) && inv != 0.f;
             if (inv == 0.f) q = 0u;
             if (__any_sync(0xffffffffu, doubt)) {
-                double w[8];
-                for (int i = 0; i < 8; i++) w[i] = swiglu64(v[k][i], u[k][i], a.mul);
-                q = exact8<NVF>(w, sb);
+                bool zeros = top == 0.f;
+                for (int i = 0; i < 8; i++) zeros &= v[k][i] == 0.f || u[k][i] == 0.f;
+                if (__any_sync(0xffffffffu, doubt && !zeros)) {
+                    double w[8];
+                    for (int i = 0; i < 8; i++) w[i] = swiglu64(v[k][i], u[k][i], a.mul);
+                    q = exact8<NVF>(w, sb);
+                }
             }
             store(c0 + k * step, q, sb);
         }
