@@ -508,6 +508,7 @@ bool tc_warm() {
     if (g_tc_ready) return true;
     if (!mmqtc::warm()) return false;
     g_tc_ready = tc_attr<64, false>() && tc_attr<128, false>() && tc_attr<192, false>() && tc_attr<192, true>();
+    if (!g_tc_ready) cudaGetLastError();       // the products stay on the CUDA cores; the next launch's check is its own
     return g_tc_ready;
 }
 
@@ -536,3 +537,4 @@ bool tc_product(bool nv, const MArgs &a) {
 }  // namespace fp4
 
 bool q4b_fp4_warm() { return fp4::tc_warm(); }
+void q4b_fp4_shutdown() { fp4::g_tc_ready = false; }      // (the limits are a device's: the next init asks for its own)

@@ -25,6 +25,7 @@ bool q4b_mmvq_warm();    // q4b_mmvq.cu: quantised rows of the dense 8-bit produ
 bool q4b_route_small_warm();   // q4b_decode.cu: counters of the one-launch routing
 void q4b_route_small_shutdown();
 bool q4b_fp4_warm();           // q4b_fp4_tc.cu: shared-memory limits of the tensor-core products
+void q4b_fp4_shutdown();
 bool q4b_balance_warm();       // q4b_balance.cu: sums of the balance loss
 void q4b_balance_shutdown();
 void q4b_mmvq_shutdown();
@@ -354,6 +355,7 @@ extern "C" void q4_hip_shutdown(void) {
     q4b_elem_shutdown();
     q4b_mmvq_shutdown();
     q4b_route_small_shutdown();
+    q4b_fp4_shutdown();
     q4b_balance_shutdown();
     q4b_fused_shutdown();
     q4b_stack_forget_host(nullptr);
