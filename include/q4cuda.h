@@ -679,7 +679,9 @@ bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_rows, uint64_
  *   d_dlogits [n_tok][n_exp] = g * d loss / d logits = g coef n_exp / n * p_tj (f_j - sum_e f_e p_te), zeros for padding;
  *   g = *d_gout (NULL: 1); d_dlogits may be d_logits
  * Any of the four may be NULL.  n_exp <= 1024, topk <= 64, n_tok < 2^23.  A row whose logits are all -inf has no
- * probabilities and no gradient; without any token that counts all results are zeros.  The same inputs give the same bits. */
+ * probabilities and no gradient; without any token that counts all results are zeros.  The same inputs give the same bits.
+ * The sums' scratch is one for all calls: graphs that hold one are replayed one after another, on whatever streams.  false also where
+ * it could not be had at q4_hip_init. */
 bool q4_cuda_route_balance(const float *d_logits, const int32_t *d_ids, const uint8_t *d_valid, uint32_t n_tok,
                            uint32_t n_exp, uint32_t topk, float coef, const float *d_gout, int32_t *d_counts,
                            float *d_prob, float *d_loss, float *d_dlogits);

@@ -256,24 +256,27 @@ template <int NV, bool VEC> bool launch(const Args &a, uint32_t clusters, uint32
 }
 }  // namespace balance
 
-// The sums' scratch, once: calls come one after another on the library's stream.
-bool q4b_balance_warm() {
-    using namespace balance;
-    if (g_done) return true;
-    uint32_t n = 0;
-    if (!launch<16, true>(Args{}, 1u, &n)) return false;
-    Q4B_CHECK(cudaMalloc(&g_part, (size_t)n * MAX_E * sizeof(float)));
-    Q4B_CHECK(cudaMalloc(&g_done, 256));
-    Q4B_CHECK(cudaMemset(g_done, 0, 256));
-    g_clusters = n;
-    return true;
-}
+// The sums' scratch, once: calls come one after another on the library's stream.  Where it cannot be had, the rest of the library
+// works without: nothing is held, no error is left, and the call refuses.
 void q4b_balance_shutdown() {
     using namespace balance;
     cudaFree(g_done);
     cudaFree(g_part);
     g_done = nullptr;
     g_part = nullptr;
+}
+bool q4b_balance_warm() {
+    using namespace balance;
+    if (g_done) return true;
+    uint32_t n = 0;
+    if (launch<16, true>(Args{}, 1u, &n) && cudaMalloc(&g_part, (size_t)n * MAX_E * sizeof(float)) == cudaSuccess &&
+        cudaMalloc(&g_done, 256) == cudaSuccess && cudaMemset(g_done, 0, 256) == cudaSuccess) {
+        g_clusters = n;
+        return true;
+    }
+    q4b_balance_shutdown();
+    cudaGetLastError();
+    return false;
 }
 
 extern "C" bool q4_cuda_route_balance(const float *d_logits, const int32_t *d_ids, const uint8_t *d_valid, uint32_t n_tok, uint32_t n_exp, uint32_t topk,

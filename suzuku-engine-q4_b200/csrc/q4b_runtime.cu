@@ -250,8 +250,8 @@ bool alloc_scratch() {
     q4b_router_tc_warm();
     q4b_mmq_tc_warm();  // without it the grouped product stays on the CUDA cores
     q4b_fp4_warm();     // ... and so do those of 4-bit floating point
-    return q4b_fused_warm() && q4b_window_warm() && q4b_elem_warm() && q4b_mmvq_warm() && q4b_route_small_warm() &&
-           q4b_balance_warm();
+    q4b_balance_warm(); // without it q4_cuda_route_balance refuses
+    return q4b_fused_warm() && q4b_window_warm() && q4b_elem_warm() && q4b_mmvq_warm() && q4b_route_small_warm();
 }
 
 }  // namespace

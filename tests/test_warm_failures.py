@@ -68,3 +68,36 @@ def test_limits_are_asked_for_again_after_a_shutdown():
     text = open(os.path.join(CSRC, "q4b_fp4_tc.cu")).read()
     assert re.search(r"void q4b_fp4_shutdown\(\) \{ fp4::g_tc_ready = false; \}", text)
     assert "q4b_fp4_shutdown();" in _function("q4b_runtime.cu", 'extern "C" void q4_hip_shutdown(void) {')
+
+
+@pytest.mark.parametrize("fail_at", range(4))
+def test_scratch_of_the_balance_loss(tmp_path, fail_at):
+    """Scratch that cannot be had: the library starts all the same, nothing is held, no error is left, and a second start tries again."""
+    text = open(os.path.join(CSRC, "q4b_balance.cu")).read()
+    macro = open(os.path.join(CSRC, "q4b_internal.cuh")).read()
+    macro = macro[macro.index("#define Q4B_CHECK"):macro.index("while (0)\n") + 10]
+    warms = ("router_tc", "mmq_tc", "fp4", "fused", "window", "elem", "mmvq", "route_small")
+    _run(tmp_path, FAKES + macro + r"""
+namespace balance {
+constexpr uint32_t MAX_E = 1024;
+struct Args {};
+static uint32_t *g_done = nullptr;
+static float *g_part = nullptr;
+static uint32_t g_clusters = 0;
+template <int NV, bool VEC> static bool launch(const Args &, uint32_t, uint32_t *most) { return step() == cudaSuccess && (*most = 18); }
+}
+""" + "".join(_function("q4b_balance.cu", h) for h in sorted(("bool q4b_balance_warm() {", "void q4b_balance_shutdown() {"), key=text.index))
+         + "".join("static bool q4b_%s_warm() { return true; }\n" % w for w in warms) + r"""
+constexpr uint32_t Q4B_XQ_SLICES = 1, Q4B_XQ_MAXLEN = 64, Q4B_MAX_TOK = 1;
+struct Q4bState { int8_t *xq; float *xd; int32_t *xbs; float *xn, *logits; int32_t *r_ids; float *r_wts; int32_t *r_cnt; float *hbuf; };
+static Q4bState g_q4b = {};
+""" + _function("q4b_runtime.cu", "bool alloc_scratch() {") + r"""
+int main() {
+    fail_at = 9 + %d;                    // behind the nine buffers of the other calls
+    if (!alloc_scratch()) return 1;
+    if (calls <= fail_at) return 2;
+    if (balance::g_done || balance::g_part || held != 9 || cudaGetLastError() != cudaSuccess) return 3;
+    fail_at = -1;
+    return q4b_balance_warm() && balance::g_done && balance::g_part && balance::g_clusters == 18 ? 0 : 4;
+}
+""" % fail_at)
