@@ -111,17 +111,18 @@ template <int NV, bool VEC> __global__ void __launch_bounds__(32u * warps(NV)) r
     int32_t n_live = 0;
 #pragma unroll
     for (uint32_t c = 0; c < CL; c++) n_live += (int32_t)peer_word(&n_here, c);
-    const float inv_n = n_live ? 1.f / (float)n_live : 0.f, share = n_live ? 1.f / ((float)n_live * (float)a.topk) : 0.f;
+    // (quotients, not products with rounded inverses: one an expert, and one a launch; no token that counts: 0 / 1)
+    const float n_f = n_live ? (float)n_live : 1.f, picks = n_f * (float)a.topk;
     for (uint32_t i = threadIdx.x; i < N; i += blockDim.x) {
         int32_t n = 0;
         if (i < a.n_exp)
 #pragma unroll
             for (uint32_t c = 0; c < CL; c++) n += (int32_t)peer_word(&hist[i], c);
         total[i] = n;
-        f[i] = (float)n * share;
+        f[i] = n_live ? __fdiv_rn((float)n, picks) : 0.f;
     }
     __syncthreads();
-    const float g = (a.gout ? *a.gout : 1.f) * a.coef * (float)a.n_exp * inv_n;
+    const float g = __fdiv_rn((a.gout ? *a.gout : 1.f) * a.coef * (float)a.n_exp, n_f);
     float acc[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) acc[i] = 0.f;
@@ -213,7 +214,7 @@ template <int NV, bool VEC> __global__ void __launch_bounds__(32u * warps(NV)) r
 #pragma unroll
                 for (uint32_t c = 0; c < 16u; c++) s += p[c];
             }
-        const float p = s * inv_n;
+        const float p = __fdiv_rn(s, n_f);
         if (a.counts) a.counts[e] = total[e];
         if (a.prob) a.prob[e] = p;
         l = fmaf(f[e], p, l);

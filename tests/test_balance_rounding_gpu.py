@@ -1,0 +1,34 @@
+"""q4_cuda_route_balance: how many roundings its results have.  Inputs with which every step but the looked-at one is exact."""
+import numpy as np
+import pytest
+
+from test_balance_gpu import EPS, call, plain
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [1, 7, 41, 47, 55, 61, 82, 83, 107, 1000, 3001])
+def test_equal_logits_give_the_fractions_themselves(dev, n):
+    """64 equal logits: probabilities of 1/64, whose sums are exact; all picks on expert 0: f is 1, the mean 1/64, the loss 64 * 1/64, whatever
+    n is.  A mean that is a product with 1/n is not, for most of these n."""
+    e = 64
+    logits, ids = np.zeros((n, e), np.float32), np.zeros((n, 1), np.int32)
+    counts, prob, loss, grad = call(dev, logits, ids, None, 1.0)
+    assert counts[0] == n and (counts[1:] == 0).all()
+    assert (prob == np.float32(1 / 64)).all() and loss == 1.0
+    # a gradient has one division, 64 / n, and one product that is not exact: 63/64 or 1/64 of it
+    want = plain(logits, ids, None, 1.0)[3]
+    assert (np.abs(grad - want) <= 2.01 * EPS * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("n,k", [(3, 7), (41, 3), (1000, 10), (4099, 6)])
+def test_shares_are_quotients(dev, n, k):
+    """One expert takes all of the probability: its mean is 1 and the loss e f, rounded once for f = counts / (n k) and then exact (e = 32)."""
+    rng = np.random.default_rng(n)
+    e = 32
+    logits = np.full((n, e), -np.inf, np.float32)
+    logits[:, 5] = rng.standard_normal(n)
+    ids = rng.integers(0, e, (n, k)).astype(np.int32)
+    counts, prob, loss, _ = call(dev, logits, ids, None, 1.0)
+    assert prob[5] == 1.0 and (np.delete(prob, 5) == 0).all()
+    assert loss == np.float32(e) * (np.float32(counts[5]) / np.float32(n * k))
