@@ -473,7 +473,7 @@ template <bool NVF, uint32_t BN, bool PAIR> bool tc_launch(const MArgs &a, uint6
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
     const cuuint64_t xd[2] = {a.cols / 2u, a.x_rows}, xs[1] = {a.cols / 2u};
-    const cuuint64_t wd[3] = {a.cols / 2u, a.w_rows, a.n_expert}, ws[2] = {a.cols / 2u, a.stride ? a.stride : code_bytes(a.w_rows, a.cols)};
+    const cuuint64_t wd[3] = {a.cols / 2u, a.w_rows, a.n_expert}, ws[2] = {a.cols / 2u, a.n_expert > 1u ? a.stride : code_bytes(a.w_rows, a.cols)};
     const cuuint32_t xb[2] = {128, 128}, x32b[2] = {128, 32}, wb[3] = {128, C::BH, 1};
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     if (!encode(&maps.x, u8, 2, a.x, xd, xs, xb) || !encode(&maps.x32, u8, 2, a.x, xd, xs, x32b) || !encode(&maps.w, u8, 3, a.w, wd, ws, wb)) return false;
