@@ -670,6 +670,8 @@ bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_rows, uint64_
                         uint32_t n_expert, const void *d_xq, uint64_t xq_rows, const int32_t *d_rows,
                         const int32_t *d_bounds, uint64_t total_rows, float scale, const float *d_expert_scale,
                         float *d_dst, uint64_t ld_dst);
+/* Products enqueued since the library was loaded: [0] on the CUDA cores, [1] on the tensor cores by single CTAs, [2] by pairs of them. */
+void q4_cuda_fp4_products(uint64_t count[3]);
 
 /* How evenly a router spreads its tokens (no reference counterpart).  d_logits [n_tok][n_exp] are the router's, d_ids
  * [n_tok][topk] the picks of q4_hip_route_pf (an id outside [0, n_exp) is no pick); d_valid [n_tok] (bytes; NULL = all)

@@ -218,6 +218,7 @@ SIGNATURES = {
     "q4_cuda_fp4_values": (b, [u32, u32, vp, u64, u64, vp, u64]),
     "q4_cuda_fp4_mul": (b, [u32, vp, u64, u64, vp, u64, f32, vp, u64]),
     "q4_cuda_fp4_mul_id": (b, [u32, vp, u64, u64, u64, u32, vp, u64, vp, vp, u64, f32, vp, vp, u64]),
+    "q4_cuda_fp4_products": (None, [vp]),
     "q4_cuda_route_balance": (b, [vp, vp, vp, u32, u32, u32, f32, vp, vp, vp, vp, vp]),
     "q4_cuda_synth_iq3s": (b, [vp, u64, u64]),
     "q4_cuda_synth_iq3s_at": (b, [vp, u64, u64, u64]),

@@ -9,6 +9,7 @@
 // values in MXFP4, 64 in NVFP4), for cols rounded up to a multiple of 256 (zero bytes there):
 //   rows     [word][row]: a product's tiles of activations begin at any row, or gather their rows
 //   weights  [row / 128][word][row % 32][row / 32 % 4]: 512 bytes that go to tensor memory as they are
+#include <atomic>
 #include <type_traits>
 
 namespace fp4 {
@@ -521,6 +522,7 @@ template <bool SWIGLU> bool quantize(uint32_t type, uint32_t form, const float *
 
 bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
 static bool g_tc_ready = false;
+static std::atomic<uint64_t> g_ran[3];         // products enqueued: CUDA cores, tensor cores by single CTAs, by pairs
 
 // Few rows on the CUDA cores while their work is that of two CTAs of 2048 columns an SM, else on the tensor cores.  us with the
 // quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 6.6, 2 rows 6.5 / 6.6, 3 rows 9.1 / 6.6;
@@ -533,6 +535,7 @@ bool product(uint32_t type, MArgs &a) {
     if (type == NV) q4b_launch(few_k<true>, grid, dim3(256), 0, g_q4b.stream, a);
     else q4b_launch(few_k<false>, grid, dim3(256), 0, g_q4b.stream, a);
     g_q4b_launches++;
+    g_ran[0]++;
     return q4b_launch_ok("fp4 product");
 }
 
@@ -651,4 +654,8 @@ extern "C" bool q4_cuda_fp4_mul_id(uint32_t type, const void *d_w, uint64_t w_ro
     a.ld = ld_dst;
     a.err = g_q4b.err_d;
     return product(type, a);
+}
+
+extern "C" void q4_cuda_fp4_products(uint64_t count[3]) {
+    for (int i = 0; count && i < 3; i++) count[i] = fp4::g_ran[i].load();
 }

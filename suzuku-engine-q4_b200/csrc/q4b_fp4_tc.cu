@@ -497,6 +497,7 @@ template <bool NVF, uint32_t BN, bool PAIR> bool tc_launch(const MArgs &a, uint6
     cfg.numAttrs = PAIR ? 2 : 1;
     (void)cudaLaunchKernelEx(&cfg, tc_k<NVF, BN, PAIR>, a, maps, vec);
     g_q4b_launches++;
+    g_ran[PAIR ? 2 : 1]++;
     return q4b_launch_ok("fp4 product");
 }
 
