@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_balance_gpu import EPS, call, plain
+from test_balance_gpu import EPS, call, inputs, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,28 @@ def test_shares_are_quotients(dev, n, k):
     counts, prob, loss, _ = call(dev, logits, ids, None, 1.0)
     assert prob[5] == 1.0 and (np.delete(prob, 5) == 0).all()
     assert loss == np.float32(e) * (np.float32(counts[5]) / np.float32(n * k))
+
+
+@pytest.mark.parametrize("t,e,k", [(64, 512, 10), (777, 64, 2), (20000, 96, 3), (20000, 600, 4), (300000, 40, 2), (2 ** 23 - 1, 2, 1)])
+def test_means_of_many_tokens(dev, t, e, k):
+    """Half steps of a mean: a warp adds up its rows one by one.  A cluster is 8 CTAs of 32 warps (24 of more than 128 experts, 16 of more
+    than 512); there are as many as the tokens need, all of up to 8 at least on any B200.  Then come its CTA's other half and 16 warps, 8
+    CTAs, 148 / 8 clusters and the division.  A probability: as in test_balance_gpu.check."""
+    rng = np.random.default_rng(t)
+    logits, ids, valid = inputs(rng, t, e, k)
+    counts, prob, loss, grad = call(dev, logits, ids, valid, 0.01, 0.5)
+    coef = float(np.float32(0.01))
+    want = plain(logits, ids, valid, coef, 0.5)
+    warps = 32 if e <= 128 else 24 if e <= 512 else 16
+    per_cluster = 8 * warps
+    rows = -(-t // (per_cluster * min(-(-t // per_cluster), 8)))
+    live = logits[valid != 0].astype(np.float64)
+    spread = (live.max(axis=1) - live.min(axis=1)).max()
+    per_p = (1.34 * spread + e / 32 + 16) * EPS
+    mean = (rows + 1 + 16 + 8 + 19 + 1) * EPS
+    assert (counts == want[0]).all()
+    assert (np.abs(prob - want[1]) <= (per_p + mean) * want[1]).all()
+    assert abs(loss - want[2]) <= (per_p + mean + (e / 32 + 20) * EPS) * want[2]
+    size = 0.5 * coef * e / len(live) * want[4] * (want[5] + (want[4] @ want[5])[:, None])
+    assert (np.abs(grad - want[3]) <= (2 * per_p + (e / 32 + 16) * EPS) * size + 1e-44).all()
+    assert dev.lib.q4_cuda_device_error() == 0
