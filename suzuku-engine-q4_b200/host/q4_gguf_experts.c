@@ -21,7 +21,7 @@ uint64_t q4b_gguf_row_bytes(uint32_t type, uint64_t ncols) {
         {0, 1, 4},    {1, 1, 2},     {2, 32, 18},   {3, 32, 20},   {6, 32, 22},   {7, 32, 24},   {8, 32, 34},
         {9, 32, 36},  {10, 256, 84}, {11, 256, 110}, {12, 256, 144}, {13, 256, 176}, {14, 256, 210},
         {15, 256, 292}, {16, 256, 66}, {17, 256, 74}, {18, 256, 98}, {19, 256, 50}, {20, 32, 18},
-        {21, 256, 110}, {22, 256, 82}, {23, 256, 136}, {30, 1, 2}};
+        {21, 256, 110}, {22, 256, 82}, {23, 256, 136}, {30, 1, 2}, {39, 32, 17}};
     for (size_t i = 0; i < sizeof T / sizeof T[0]; i++)
         if (T[i].type == type) return (ncols % T[i].per) ? 0 : ncols / T[i].per * T[i].bytes;
     return 0;

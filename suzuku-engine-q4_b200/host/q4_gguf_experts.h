@@ -23,7 +23,7 @@ typedef struct q4b_gguf_tensor {
     char name[128];
     uint32_t n_dims;
     uint64_t ne[4];         /* ne[0] = columns (fastest), ne[1] = rows, ne[2] = experts */
-    uint32_t type;          /* ggml type id (IQ3_S = 21, IQ4_NL = 20, IQ4_XS = 23, F32 = 0) */
+    uint32_t type;          /* ggml type id (IQ3_S = 21, IQ4_NL = 20, IQ4_XS = 23, MXFP4 = 39, F32 = 0) */
     uint64_t offset;        /* from the start of the data section */
     uint64_t nbytes;
 } q4b_gguf_tensor;

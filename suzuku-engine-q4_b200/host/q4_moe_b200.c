@@ -81,6 +81,7 @@ bool q4b_moe_layer_load_gguf(q4b_moe_layer *L, int arena, const void *gguf, int3
     uint64_t og, ou, od, pb;
     uint32_t n_expert;
     if (!L || !q4b_gguf_expert_parts(g, layer, &tg, &tu, &td, &og, &ou, &od, &pb, &n_expert)) return false;
+    if (tg->type == Q4_T_MXFP4 || tu->type == Q4_T_MXFP4 || td->type == Q4_T_MXFP4) return false;
     uint8_t *stage = (uint8_t *)q4_hip_host_alloc_coh(2 * pb);
     if (!stage) return false;
     const bool sh = q4b_gguf_read_shared_pack(g, layer, stage, pb) == (int64_t)pb;

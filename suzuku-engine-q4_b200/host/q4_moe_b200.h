@@ -52,8 +52,9 @@ bool q4b_moe_layer_load_stacked(q4b_moe_layer *L, int arena, const uint8_t *gate
 /* The same from a GGUF model file (host/q4_gguf_experts.h): the layer's stacked expert tensors
  * are sliced into packs expert by expert (src/q4_expert.c:962-993) and uploaded, the shared
  * expert's tensors (if the layer has them) into the slot after the last routed expert.  The
- * shapes come from the tensors.  Takes any pack the file holds; the arena is tiled only when
- * the pack is all IQ3_S.  `gguf` is a q4b_gguf the caller opened. */
+ * shapes come from the tensors.  Takes any pack the file holds but MXFP4 ones, whose products do not
+ * read arenas (q4_cuda_fp4_put takes their packs); the arena is tiled only when the pack is all
+ * IQ3_S.  `gguf` is a q4b_gguf the caller opened. */
 bool q4b_moe_layer_load_gguf(q4b_moe_layer *L, int arena, const void *gguf, int32_t layer);
 
 /* Scratch floats q4_moe_layer_dev needs at d_ws (src/q4_moe.c:2062-2065 sizes it the same way). */
