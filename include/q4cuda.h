@@ -650,7 +650,9 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  *                    only p below total_rows), = scale * d_expert_scale[e] * W_e . x[d_rows[p]]; d_expert_scale NULL = 1, d_rows NULL
  *                    = p itself, an entry of d_rows outside [0, xq_rows) gives a row of zeros.  Rows of d_dst that no
  *                    expert has are left alone.  n_expert <= 1024
- * Sums are fp32; products of codes are exact.  Outputs may not overlap inputs. */
+ * Sums are fp32; products of codes are exact.  Outputs may not overlap inputs.  The products run on the CUDA cores with few rows and on
+ * the tensor cores with more, which add up in another order: a row's last bits may depend on how many rows the call has (q4_mmvq_n's do
+ * not), by no more than the sums' own rounding. */
 #define Q4_T_MXFP4 39u
 #define Q4_T_NVFP4 40u
 #define Q4_FP4_ROWS 0u

@@ -524,13 +524,20 @@ bool tc_product(bool nv, const MArgs &a);      // q4b_fp4_tc.cu
 static bool g_tc_ready = false;
 static std::atomic<uint64_t> g_ran[3];         // products enqueued: CUDA cores, tensor cores by single CTAs, by pairs
 
-// Few rows on the CUDA cores while their work is that of two CTAs of 2048 columns an SM, else on the tensor cores.  us with the
-// quantiser ahead, weights from HBM (CUDA cores / tensor cores): 4096 x 2048 1 row 6.3 / 6.6, 2 rows 6.5 / 6.6, 3 rows 9.1 / 6.6;
-// 8192 x 2560 1 row 8.5 / 7.6; 1024 x 1024 1 row 3.9 / 5.1, 8 rows 4.4 / 5.2.
+// Few rows on the CUDA cores while they are at most two CTAs an SM, counted as often as one has 2048 columns, else on the tensor cores.
+// us with the quantiser ahead, MXFP4, the first line's weights from HBM, the others' from the L2 (CUDA cores / tensor cores):
+//   4096 x 2048   1 row 5.9 / 6.1, 2 rows 6.1 / 6.1, 3 rows 8.7 / 6.2
+//   1024 x 1024   1 row 3.8 / 5.0, 8 rows 4.4 / 5.2, 12 rows 6.1 / 5.2, 18 rows 6.8 / 5.3
+//   512 x 2048    1 row 4.6 / 5.8, 18 rows 6.1 / 6.1, 19 rows 8.3 / 6.1
+//   8192 x 128    1 row 4.3 / 4.4, 8 rows 19.3 / 4.6
+//   128 x 4096    8 rows 7.3 / 7.7, 37 rows 8.6 / 8.0
+//   256 x 256     32 rows 4.4 / 4.5, 128 rows 11.0 / 5.3
+//   64 x 128      32 rows 3.8 / 4.4, 128 rows 5.7 / 5.1, 1184 rows 31.6 / 5.3
+// The two add a row up in different orders: its last bits change with the rows beside it where their number crosses the line.
 bool product(uint32_t type, MArgs &a) {
     OnDevice dev;
     const uint64_t ctas = a.total * ((a.w_rows + 127u) / 128u * 4u);
-    if (g_tc_ready && ctas * a.cols > 2u * (uint64_t)g_q4b.n_sm * 2048u) return tc_product(type == NV, a);
+    if (g_tc_ready && ctas * (a.cols < 2048u ? 2048u : a.cols) > 2u * (uint64_t)g_q4b.n_sm * 2048u) return tc_product(type == NV, a);
     const dim3 grid((a.w_rows + 127u) / 128u * 4u, (unsigned)(a.total < 65535u ? a.total : 65535u));
     if (type == NV) q4b_launch(few_k<true>, grid, dim3(256), 0, g_q4b.stream, a);
     else q4b_launch(few_k<false>, grid, dim3(256), 0, g_q4b.stream, a);

@@ -123,3 +123,20 @@ def test_blocks_without_a_number(dev, ty, rows, kind):
     assert nan.sum() == 2 * w_rows + 3 * rows - 6 and (np.isnan(y) == nan).all()
     bound = F.product_bound(np.nan_to_num(xv), np.nan_to_num(wv), 1.0, cols // F.BLOCK[ty])
     assert (np.abs(y - want)[~nan] <= bound[~nan]).all()
+
+
+@pytest.mark.parametrize("w_rows,cols,rows,kind", [(64, 128, 32, 0), (64, 128, 1184, 1), (1000, 32, 9, 0), (1000, 32, 64, 1), (8192, 128, 1, 0), (8192, 128, 8, 1),
+                                                   (1024, 1024, 8, 0), (1024, 1024, 12, 1), (128, 4096, 8, 0), (128, 4096, 75, 1)])
+def test_narrow_matrices_leave_the_cuda_cores_in_time(dev, w_rows, cols, rows, kind):
+    """A CTA of the CUDA cores' kernel costs about the same with 32 columns as with 2048: what counts is how many there are."""
+    lib, ty = dev.lib, F.MXFP4
+    rng = np.random.default_rng(rows)
+    w, d_w = _weights(dev, rng, ty, w_rows, cols)
+    x, d_x = _rows(dev, rng, ty, rows, cols)
+    d_y = dev.malloc(rows * w_rows * 4)
+    before = _ran(dev)
+    assert lib.q4_cuda_fp4_mul(ty, d_w, w_rows, cols, d_x, rows, 1.0, d_y, w_rows)
+    assert _ran(dev, before) == [int(i == kind) for i in range(3)]
+    y = dev.download(d_y, (rows, w_rows), np.float32)
+    assert (np.abs(y - x @ w.T) <= F.product_bound(x, w, 1.0, cols // 32)).all()
+    assert lib.q4_cuda_device_error() == 0
