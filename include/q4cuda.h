@@ -631,8 +631,9 @@ bool q4_cuda_mmq_q8_sections(const void *xq, uint64_t rows, uint64_t cols, const
  *   Q4_T_NVFP4  16 values share an e4m3 number; byte 0x7f = NaN.  A factor for a whole matrix, where there is one, is
  *               the caller's and goes into the products' scale
  * Quantising v = x * mul (rounded to fp32): MXFP4 takes the power of two floor(log2 max|v|) - 2 (-127 at least), NVFP4 the
- * e4m3 number nearest to max|v| times fp32's 1/6 (448 at most; where that is 0, so is the block); codes are the nearest,
- * ties to even, 6 for all beyond it.  A block with an infinity or a NaN becomes NaN.
+ * e4m3 number nearest to max|v| times fp32's 1/6 (an fp32 product; 448 at most; where that is 0, so is the block); codes are the nearest,
+ * ties to even, 6 for all beyond it.  (swiglu_quantize, whose values are no fp32 numbers, takes max / 6: the two differ for one fp32
+ * max a binade, whose sixth is half-way between two e4m3 numbers to within that product's rounding.)  A block with an infinity or a NaN becomes NaN.
  * cols: a multiple of 32, at most 65536; any number of rows below 2^31.  A quantised matrix is an opaque
  * buffer of q4_cuda_fp4_bytes(type, form, rows, cols) bytes (0: not a shape of these), 16-byte aligned, in one of two forms:
  *   Q4_FP4_ROWS     activations: what the products take as d_xq

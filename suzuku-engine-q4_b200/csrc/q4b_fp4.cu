@@ -69,7 +69,9 @@ __device__ __forceinline__ float e8m0_value(uint32_t b) {
 template <bool NVF> __device__ __forceinline__ float scale_value(uint32_t b) { return NVF ? e4m3_value(b) : e8m0_value(b); }
 
 // The scale byte of a block whose largest magnitude is a.  MXFP4: the power of two that brings a into [4, 8); NVFP4: a sixth
-// of a (its product with fp32's 1/6), rounded to e4m3.
+// of a, rounded to e4m3.  The sixth is the fp32 product with fp32's 1/6, off by 1.5 * 2^-24 at most, as fp32 frameworks divide by a
+// constant on a GPU: rows that one of them quantises get the same bytes.  A quotient would name another scale for one fp32 number a
+// binade, 7.125 less a step times a power of two, whose sixth lies between two e4m3 numbers to within that rounding.
 template <bool NVF> __device__ __forceinline__ uint32_t scale_byte(float a) {
     if (!(a <= 3.402823466e38f)) return NVF ? 0x7fu : 255u;
     if (NVF) return e4m3_nearest(a * (1.f / 6.f));
