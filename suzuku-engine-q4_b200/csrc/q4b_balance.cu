@@ -73,8 +73,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // memory.  Then a warp takes a token's row at a time, 32 NV experts in registers (VEC: four neighbours a lane and load); its sums
 // of probabilities stay there too.  They are added up in a fixed order: over the warps of a CTA in shared memory, over the
 // CTAs of a cluster (each takes an eighth of the experts), over the clusters by the last CTA to come to its end.  A chain of
-// short steps: 8192 x 512, top-10, 16.1 us, of them counts 3, rows 5.8 (5.8 TB/s), sums and their barriers 5; 64 x 512 8.4.  (Four
-// launches, with counts by global atomics, took 33.6 and 10.5.)
+// short steps: 8192 x 512, top-10, 16.1 us with inputs in the L2 and 17.5 with three sets of inputs in turn, of them counts 3, rows 5.8
+// (5.8 TB/s), sums and their barriers 5; 64 x 512 8.4.  (Four launches, with counts by global atomics, took 33.6 and 10.5.)
 // Warps of a CTA: as many as have registers for a row and its sums.
 __host__ __device__ constexpr uint32_t warps(int nv) { return nv > 16 ? 16u : nv > 4 ? 24u : 32u; }
 template <int NV, bool VEC> __global__ void __launch_bounds__(32u * warps(NV)) rows_k(const Args a) {

@@ -186,8 +186,9 @@ template <bool NVF> __device__ __noinline__ uint32_t exact8(const double *v, uin
 }
 
 // A warp takes 256 values of a row at a time, eight a lane: a block is two or four lanes.  The eight warps of a CTA take the same
-// columns of eight rows that follow one another; U such pieces of a row are loaded before the first is quantised (two of 8192 x 2048 14.6 us, 5.3 TB/s; one 16.4, four 16.0; with SwiGLU 22528 x 512 two 19.4 us,
-// 5.1 TB/s, one 20.3).  Bound by those loads and, with SwiGLU, by issue slots.
+// columns of eight rows that follow one another; U such pieces of a row are loaded before the first is quantised (short runs: two of
+// 8192 x 2048 14.6 us, 5.3 TB/s; one 16.4, four 16.0; with SwiGLU 22528 x 512 two 19.4 to 20.0 us, 5.0 to 5.1 TB/s, one 20.3; two over
+// 0.3 s 15.0 and 20.5).  Bound by those loads and, with SwiGLU, by issue slots.
 template <bool NVF, bool WF, bool SWIGLU, bool VEC> __global__ void __launch_bounds__(256) quantize_k(const QArgs a) {
     constexpr int U = 2;
     q4b_pdl_wait();

@@ -10,9 +10,10 @@
 //   warp 12     brings a stage's scales to tensor memory (tcgen05.cp) and issues its MMAs
 //   warps 4-11  read a finished accumulator, apply the factor and store, while the MMAs fill the other one: 32 x 32 at a time
 //               through shared memory (TMA), of fewer rows from the registers
-// What bounds it: with few rows an expert the reads of W (64 tokens, top-10 of 512 experts, 1024 x 2048, NVFP4: 73 us, 5.9 TB/s); with
-// many the loads of a stage, 35 to 45 KB that arrive at some 45 bytes a cycle and SM, beside the stores of fp32 results (8192 x 4096 x
-// 2048, NVFP4: 47 us, 2.9 PFLOP/s, tensor pipe 39 %), hence tiles as large as two accumulators and the scales leave room for.
+// What bounds it: with few rows an expert the reads of W (64 tokens, top-10 of 512 experts, 1024 x 2048, NVFP4: 71 to 73 us, 5.9 TB/s,
+// in a short run of calls; 80 over 0.3 s, which the power cap slows down); with many the loads of a stage, 35 to 45 KB that arrive
+// at some 45 bytes a cycle and SM, beside the stores of fp32 results (8192 x 4096 x 2048, NVFP4: 47 to 48 us in a short run, 2.9
+// PFLOP/s, tensor pipe 39 %; 55 over 0.3 s), hence tiles as large as two accumulators and the scales leave room for.
 // Scales in tensor memory: 128 rows' words are 4 columns (row r in lane r % 32 of column r / 32, copied to the four lane
 // quarters), a word serves 128 values of k in MXFP4 (two MMAs, told apart in the instruction descriptor), 64 in NVFP4.
 namespace fp4 {
@@ -517,7 +518,7 @@ template <uint32_t BN, bool PAIR> bool tc_go(bool nv, const MArgs &a, uint64_t m
     return nv ? tc_launch<true, BN, PAIR>(a, m_tiles) : tc_launch<false, BN, PAIR>(a, m_tiles);
 }
 // The tile of 64, 128 or 192 rows of W with which the busiest SM has least to do: its rows and 96 for a tile's beginning and end
-// (of 64 / 128 / 192, us: 777 rows x 4099 x 2560 17 / 13.6 / 15.5; 64 tokens, top-10 of 512 experts, 1024 x 2048 127 / 75 / 73;
+// (short runs; of 64 / 128 / 192, us: 777 rows x 4099 x 2560 17 / 13.6 / 15.5; 64 tokens, top-10 of 512 experts, 1024 x 2048 127 / 75 / 73;
 // one token of them 8.7 / 6.8 / 8.0; 8192 tokens 380 / 243 / 209).  Pairs of CTAs, which halve the reads of W, for dense products of
 // four rounds of tiles and more: 8192 x 4096 x 2048 47.1 us, by single CTAs 52.0.  Of experts with fewer than 256 rows half a pair
 // idles (the 8192 tokens above: 259 us).
